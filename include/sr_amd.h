@@ -350,6 +350,71 @@ int sr_fdconv_weightgen_backward(int B, const float* pooled, int pooled_ld, cons
                                  const sr_weight_path_grads* grads, float* dpooled, int dpooled_ld, int accumulate,
                                  void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- optimizer: AdamW over many tensors, global gradient norm -------------------------------------------------------------
+ * Takes over optimizer.step() and clip_grad_norm_ of the training scripts (train/train_realESRGAN_fdconv_1.py:118,
+ * train/train_realESRGAN_fdconv.py:142) for parameter lists of any length, with decoupled weight decay, moments in float32 or in
+ * 8 bits, and the weight average (`params_ema`) of the Real-ESRGAN recipe.
+ *   g = grad * factor;  m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g g
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) (1 - b2^t)^-1/2 + eps);  ema = d ema + (1-d) p
+ * in float32, one rounding per operation.  bits = 8: SR_ADAMW_BLOCK consecutive values of a tensor share an exponent byte; m is
+ * held as sign + 4 exponent + 3 mantissa bits, v as 5 + 3, rounded stochastically by a hash of (seed, step, element number), as
+ * bfloat16 parameters are.  v > 0 is never rounded to 0.  A block in which a moment is not finite decodes to NaN as a whole. */
+#define SR_ADAMW_BLOCK 256
+#define SR_ADAMW_SCALARS_BYTES 64
+#define SR_ADAMW_SKIP ((uintptr_t)1) /* in a gradient table: leave this tensor alone (NULL: no gradient, only its average moves) */
+typedef struct {
+    void* p;              /* n parameters in the list's dtype, updated in place */
+    void *m, *v;          /* moments: float[n] (bits 32) or uint8_t[n] codes (bits 8) */
+    uint8_t *me, *ve;     /* bits 8: exponent bytes, (n + 255) / 256 each; else ignored */
+    float* ema;           /* float[n] or NULL (all tensors of a list alike) */
+    int64_t n;            /* may be 0 */
+    int64_t index;        /* number of the first element among all of the optimizer's */
+} sr_adamw_tensor;
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay, ema_decay;
+    uint64_t seed;
+} sr_adamw_hyper;
+typedef struct sr_adamw sr_adamw; /* a list of tensors of one dtype and kind of moments, on one device */
+/* `tensors` is a HOST array, copied.  The tensors must not overlap.  SR_ERR_STATE from the other calls: another device is current. */
+int sr_adamw_create(int dtype, int bits, int count, const sr_adamw_tensor* tensors, sr_adamw** out);
+void sr_adamw_destroy(sr_adamw* list);
+/* One step of all tensors.  grads: device array of `count` device pointers to gradients in the list's dtype (any alignment of
+ * their elements).  factor: a device float, or NULL (1).  step: counted from 1, with `hyper`; or scalars != NULL: what sr_adamw_tick
+ * wrote (hyper and step are then ignored). */
+int sr_adamw_step(const sr_adamw* list, const sr_adamw_hyper* hyper, int64_t step, const void* scalars, const void* const* grads,
+                  const float* factor, void* stream);
+/* For captured graphs: *step += 1 and the scalars of that step, on the device; lr: a device float, or NULL (hyper->lr).
+ * scalars: SR_ADAMW_SCALARS_BYTES. */
+int sr_adamw_tick(const sr_adamw_hyper* hyper, const float* lr, int64_t* step, void* scalars, void* stream);
+/* The moments as the values they stand for: m[index + i], v[index + i] in dtype.  And back, from float32 (values that 8 bits hold stay
+ * what they are; v < 0 becomes NaN). */
+int sr_adamw_moments(const sr_adamw* list, int dtype, void* m, void* v, void* stream);
+int sr_adamw_set_moments(const sr_adamw* list, const float* m, const float* v, uint64_t seed, void* stream);
+
+/* out[0] = sqrt(sum of squares) over all lists (summed in float64 in a fixed order), out[1] = min(1, max_norm / (out[0] + 1e-6)).
+ * A list is an sr_adamw with its gradient table, or (list == NULL) a device array of spans; `lists` is a HOST array. */
+#define SR_GRAD_MAX_LISTS 64
+typedef struct {
+    void* g; /* n gradients */
+    int64_t n;
+} sr_grad_span;
+typedef struct {
+    const sr_adamw* list;
+    const void* const* grads;
+    const sr_grad_span* spans;
+    int64_t nspans;
+    int32_t dtype; /* of the spans */
+    int32_t _pad;
+} sr_grad_list;
+size_t sr_grad_norm_workspace_bytes(int nlists);
+int sr_grad_norm(int nlists, const sr_grad_list* lists, double max_norm, float* out, void* workspace, size_t workspace_bytes,
+                 void* stream);
+/* g *= *factor over device spans that do not overlap (one wave takes a span at a time: split long tensors) */
+int sr_grad_scale(int dtype, int64_t nspans, const sr_grad_span* spans, const float* factor, void* stream);
+/* Copies a small HOST array (tables of pointers) to the device through kernel arguments: by value, so the source may be reused at
+ * once and a captured graph keeps what it held; 3840 bytes per launch.  bytes and dst: multiples of 4. */
+int sr_upload(const void* src_host, void* dst, size_t bytes, void* stream);
+
 /* ---- whole network (RRDBNet.forward) ------------------------------------------------------- */
 typedef struct sr_rrdbnet sr_rrdbnet;
 int sr_rrdbnet_create(int num_in_ch, int num_out_ch, int scale, int num_feat, int num_block, int num_grow_ch,

@@ -55,6 +55,22 @@ class GateConsumer(C.Structure):
     _fields_ = [('w', C.c_void_p * 3), ('b', C.c_void_p * 3), ('logits', C.c_void_p), ('gates', C.c_void_p), ('first', C.c_int32)]
 
 
+class AdamWTensor(C.Structure):
+    _fields_ = [('p', C.c_void_p), ('m', C.c_void_p), ('v', C.c_void_p), ('me', C.c_void_p), ('ve', C.c_void_p), ('ema', C.c_void_p),
+                ('n', C.c_int64), ('index', C.c_int64)]
+
+
+class AdamWHyper(C.Structure):
+    _fields_ = [(n, C.c_double) for n in ('lr', 'beta1', 'beta2', 'eps', 'weight_decay', 'ema_decay')] + [('seed', C.c_uint64)]
+
+
+class GradList(C.Structure):
+    _fields_ = [('list', C.c_void_p), ('grads', C.c_void_p), ('spans', C.c_void_p), ('nspans', C.c_int64), ('dtype', C.c_int32),
+                ('_pad', C.c_int32)]
+
+
+ADAMW_BLOCK, ADAMW_SCALARS_BYTES, ADAMW_SKIP, GRAD_MAX_LISTS = 256, 64, 1, 64
+
 _SIGS = {
     'sr_strerror': (C.c_char_p, [C.c_int]),
     'sr_last_hip_error': (C.c_int, []),
@@ -126,6 +142,16 @@ _SIGS = {
                                      C.c_void_p, C.c_size_t, C.c_void_p]),
     'sr_rrdbnet_profile': (C.c_int, [C.c_void_p, C.c_int]),
     'sr_rrdbnet_profile_read': (C.c_int, [C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_long)]),
+    'sr_adamw_create': (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(AdamWTensor), C.POINTER(C.c_void_p)]),
+    'sr_adamw_destroy': (None, [C.c_void_p]),
+    'sr_adamw_step': (C.c_int, [C.c_void_p, C.POINTER(AdamWHyper), C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    'sr_adamw_tick': (C.c_int, [C.POINTER(AdamWHyper), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    'sr_adamw_moments': (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    'sr_adamw_set_moments': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    'sr_grad_norm_workspace_bytes': (C.c_size_t, [C.c_int]),
+    'sr_grad_norm': (C.c_int, [C.c_int, C.POINTER(GradList), C.c_double, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    'sr_grad_scale': (C.c_int, [C.c_int, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    'sr_upload': (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     'sr_debug_force_generic_conv': (None, [C.c_int]),
     'sr_debug_force_generic_fft': (None, [C.c_int]),
     'sr_debug_no_mixed_fft': (None, [C.c_int]),

@@ -8,8 +8,12 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
-SOURCES = ['layout.hip', 'fbm.hip', 'fbm_fast.hip', 'fbm_fast_mixed.hip', 'fbm_mfma.hip', 'gates.hip', 'weightgen.hip', 'weightgen_bwd.hip', 'conv.hip', 'conv_plain.hip', 'net.hip', 'head.hip', 'train.hip']
+SOURCES = ['layout.hip', 'fbm.hip', 'fbm_fast.hip', 'fbm_fast_mixed.hip', 'fbm_mfma.hip', 'gates.hip', 'weightgen.hip', 'weightgen_bwd.hip', 'conv.hip', 'conv_plain.hip', 'net.hip', 'head.hip', 'train.hip', 'adamw.hip']
+# adamw.hip: every operation rounded once (its results are those of the formulas, bit for bit), and no packed float32 instructions
+EXTRA = {'adamw.hip': ['-ffp-contract=off', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']}
 OUT = os.path.join(HERE, 'libsr_amd.so')
+HOST_SRC = os.path.join(CSRC, 'torch_host.cpp')
+HOST_OUT = os.path.join(HERE, 'libsr_amd_torch.so')
 
 
 def _stale():
@@ -20,9 +24,32 @@ def _stale():
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _host_command():
+    """g++ line of the small library that reads torch's tensor objects (csrc/torch_host.cpp)."""
+    import sysconfig
+    import torch
+    root = os.path.dirname(torch.__file__)
+    return ['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-Wall', '-fvisibility=hidden', '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch.compiled_with_cxx11_abi(),
+            '-isystem', os.path.join(root, 'include'), '-isystem', os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'),
+            '-isystem', sysconfig.get_paths()['include'], HOST_SRC, '-o', HOST_OUT,
+            '-L' + os.path.join(root, 'lib'), '-ltorch_python', '-ltorch_cpu', '-lc10']
+
+
 def build(force=False, verbose=True):
-    if not force and not _stale():
-        return OUT
+    host = None
+    if force or not os.path.exists(HOST_OUT) or os.path.getmtime(HOST_SRC) > os.path.getmtime(HOST_OUT):
+        cmd = _host_command()
+        host = (cmd, subprocess.Popen(cmd))
+    try:
+        if force or _stale():
+            _build_kernels(force, verbose)
+    finally:
+        if host and host[1].wait() != 0:
+            raise RuntimeError('g++ failed: ' + ' '.join(host[0]))
+    return OUT
+
+
+def _build_kernels(force, verbose):
     hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
     objs = []
     procs = []
@@ -35,8 +62,8 @@ def build(force=False, verbose=True):
         src = os.path.join(CSRC, s)
         if not force and os.path.exists(o) and os.path.getmtime(o) > max(os.path.getmtime(src), newest_header):
             continue  # object is newer than its source and every header
-        cmd = [hipcc, '-O3', '--offload-arch=gfx950', '-std=c++17', '-fno-signed-zeros', '-fPIC', '-Wall', '-Wno-unused-result', '-c',
-               os.path.join(CSRC, s), '-o', o]
+        cmd = [hipcc, '-O3', '--offload-arch=gfx950', '-std=c++17', '-fno-signed-zeros', '-fPIC', '-Wall', '-Wno-unused-result'] + EXTRA.get(s, []) + [
+               '-c', os.path.join(CSRC, s), '-o', o]
         procs.append((cmd, subprocess.Popen(cmd)))
     for cmd, p in procs:
         if p.wait() != 0:
@@ -45,7 +72,6 @@ def build(force=False, verbose=True):
     subprocess.check_call(cmd)
     if verbose:
         print('built', OUT)
-    return OUT
 
 
 if __name__ == '__main__':

@@ -1,0 +1,787 @@
+// AdamW over many tensors at once, moments in 32 or in 8 bits, and the global gradient norm (include/sr_amd.h "optimizer").
+//
+// One step of a tensor, every operation rounded once to float32 (this file is compiled without contraction, so that the
+// results are those of the formulas, bit for bit):
+//   g  = grad * factor                         factor: 1, or min(1, max_norm / (norm + 1e-6)) from device memory
+//   m' = b1 m + (1 - b1) g                     v' = b2 v + (1 - b2) (g g)
+//   p' = p (1 - lr wd) - lr / (1 - b1^t) * (m' / (sqrt(v') * (1 - b2^t)^-1/2 + eps))
+//   e' = d e + (1 - d) p'                      the weight average, if there is one
+//
+// Moments in 8 bits.  256 consecutive values of a tensor (a block) share an exponent E, that of the block's largest value (one
+// more if its mantissa is above 1.875, so that no value rounds out of range).  A code is the top of the float that holds
+// x * 2^-(E + 112) (m) or x * 2^-(E + 96) (v): those floats have an exponent field of at most 15 or 31, so bits 20 and up are a
+// 4-bit exponent and 3 mantissa bits, or a 5-bit exponent and 3 mantissa bits, subnormals included; m has its sign in bit 7.
+// Both reach down to 2^-17 of the block's largest gradient (2^-33 of the largest v).  Adding 20 random bits before the cut is
+// stochastic rounding: with b2 = 0.999 v moves by a thousandth a step, a hundredth of the distance of two codes, and rounded
+// to nearest it would never move; rounded so, its mean is right.  v' > 0 does not round to 0 (m' / (sqrt(0) + eps) would be a
+// step of 1 / eps).  bfloat16 weights are rounded the same way for the same reason.  The random bits are a hash of (seed, step,
+// number of the element): no state, no order, the same on every run.  A scale that is a power of two decodes exactly, and what
+// was decoded encodes to itself, so a checkpoint in float32 resumes where it was.  A block with a NaN or an infinity has the
+// exponent byte 255 and decodes to NaN as a whole.
+//
+// What bounds it: memory.  Every value is read and written once (28 bytes of float32 state, 16 with 8-bit moments) against 40 to
+// 90 vector instructions.  Work is split into pieces of 1024 consecutive values of one tensor, one per WAVE: RRDBNet-FDConv has
+// 8380 tensors of which 8000 are smaller than a piece, and a workgroup each would leave three of its four waves idle.  A wave
+// issues the loads of its four groups of 256 values (16 bytes per lane and tensor) before it computes.
+#include "common.h"
+
+#include <math.h>
+#include <string.h>
+
+#include <new>
+#include <vector>
+
+#pragma clang fp contract(off)
+
+namespace sr {
+
+constexpr int PIECE = 1024;              // values of one wave
+constexpr int QBLOCK = SR_ADAMW_BLOCK;   // values that share an exponent
+static_assert(QBLOCK == 256, "a wave of 64 lanes holds four values each of a block");
+constexpr int NORM_WG = 2048;            // workgroups (= partial sums) of the norm per list: 8 per CU
+constexpr uint32_t GOLDEN = 0x9E3779B1u;
+
+struct Rec {  // one tensor, 64 bytes: one scalar load
+    void* p;
+    void *m, *v;
+    uint8_t *me, *ve;
+    float* ema;
+    int64_t n, index;
+};
+struct Piece {
+    uint32_t tensor, number;  // the number-th PIECE values of the tensor
+};
+
+struct Scalars {
+    float b1, c1, b2, c2, decay, step_size, rbc2, eps, d, cd;
+    uint32_t k0, k1;
+};
+
+__host__ __device__ inline void make_key(uint64_t seed, int64_t step, Scalars& s) {  // splitmix64
+    uint64_t z = seed + (uint64_t)step * 0x9E3779B97F4A7C15ull;
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    z ^= z >> 31;
+    s.k0 = (uint32_t)z;
+    s.k1 = (uint32_t)(z >> 32);
+}
+__host__ __device__ inline Scalars make_scalars(const sr_adamw_hyper& h, double lr, int64_t step) {
+    Scalars s;
+    s.b1 = (float)h.beta1;
+    s.c1 = (float)(1.0 - h.beta1);
+    s.b2 = (float)h.beta2;
+    s.c2 = (float)(1.0 - h.beta2);
+    s.decay = (float)(1.0 - lr * h.weight_decay);
+    s.step_size = (float)(lr / (1.0 - pow(h.beta1, (double)step)));
+    s.rbc2 = (float)pow(1.0 - pow(h.beta2, (double)step), -0.5);
+    s.eps = (float)h.eps;
+    s.d = (float)h.ema_decay;
+    s.cd = (float)(1.0 - h.ema_decay);
+    make_key(h.seed, step, s);
+    return s;
+}
+
+// 32 random bits for element (hi, lo) of a step; hi_c = hi * GOLDEN.  The two odd constants and the shifts are a published
+// full-avalanche mixer of 32-bit words; k1 enters between them so that steps whose k0 differ in few bits do not share values.
+__device__ __forceinline__ uint32_t mix(uint32_t lo, uint32_t hi_c, uint32_t k0, uint32_t k1) {
+    uint32_t x = (lo ^ k0) + hi_c;
+    x = (x ^ (x >> 16)) * 0x7FEB352Du + k1;
+    x = (x ^ (x >> 15)) * 0x846CA68Bu;
+    return x ^ (x >> 16);
+}
+
+// vectors with the alignment of their elements: tensors are views at any offset (the gradients of one layer are pieces of one
+// buffer); the hardware loads and stores 16 bytes at any address
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t h4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint8_t b4u __attribute__((ext_vector_type(4), aligned(1)));
+
+// 4 values at p, of which the first cnt exist (the others: 0)
+__device__ __forceinline__ void load4(const float* p, int cnt, float (&r)[4]) {
+    if (cnt >= 4) {
+        const f4u x = *(const f4u*)p;
+        r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
+    } else {
+        r[0] = cnt > 0 ? p[0] : 0.f, r[1] = cnt > 1 ? p[1] : 0.f, r[2] = cnt > 2 ? p[2] : 0.f, r[3] = 0.f;
+    }
+}
+__device__ __forceinline__ void load4(const bf16_t* p, int cnt, float (&r)[4]) {
+    if (cnt >= 4) {
+        const h4u x = *(const h4u*)p;
+        r[0] = bf16_to_f32(x.x), r[1] = bf16_to_f32(x.y), r[2] = bf16_to_f32(x.z), r[3] = bf16_to_f32(x.w);
+    } else {
+        r[0] = cnt > 0 ? bf16_to_f32(p[0]) : 0.f, r[1] = cnt > 1 ? bf16_to_f32(p[1]) : 0.f, r[2] = cnt > 2 ? bf16_to_f32(p[2]) : 0.f, r[3] = 0.f;
+    }
+}
+__device__ __forceinline__ void store4(float* p, int cnt, const float (&r)[4]) {
+    if (cnt >= 4) {
+        const f4u x = {r[0], r[1], r[2], r[3]};
+        *(f4u*)p = x;
+    } else {
+        if (cnt > 0) p[0] = r[0];
+        if (cnt > 1) p[1] = r[1];
+        if (cnt > 2) p[2] = r[2];
+    }
+}
+__device__ __forceinline__ void store4(bf16_t* p, int cnt, const uint16_t (&r)[4]) {
+    if (cnt >= 4) {
+        const h4u x = {r[0], r[1], r[2], r[3]};
+        *(h4u*)p = x;
+    } else {
+        if (cnt > 0) p[0] = r[0];
+        if (cnt > 1) p[1] = r[1];
+        if (cnt > 2) p[2] = r[2];
+    }
+}
+__device__ __forceinline__ uint32_t load4b(const uint8_t* p, int cnt) {  // byte j of the result: code j
+    if (cnt >= 4) return __builtin_bit_cast(uint32_t, *(const b4u*)p);
+    uint32_t r = 0;
+    if (cnt > 0) r = p[0];
+    if (cnt > 1) r |= (uint32_t)p[1] << 8;
+    if (cnt > 2) r |= (uint32_t)p[2] << 16;
+    return r;
+}
+__device__ __forceinline__ void store4b(uint8_t* p, int cnt, uint32_t x) {
+    if (cnt >= 4) {
+        *(b4u*)p = __builtin_bit_cast(b4u, x);
+    } else {
+        if (cnt > 0) p[0] = (uint8_t)x;
+        if (cnt > 1) p[1] = (uint8_t)(x >> 8);
+        if (cnt > 2) p[2] = (uint8_t)(x >> 16);
+    }
+}
+
+// the largest of 64 lanes' unsigned values, in all lanes (every lane must be active): rows of 16, then across the rows
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t x) {
+    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+    return x > y ? x : y;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    x = dpp_max<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+    x = dpp_max<0x112, 0xf>(x);
+    x = dpp_max<0x114, 0xf>(x);
+    x = dpp_max<0x118, 0xf>(x);
+    x = dpp_max<0x142, 0xa>(x);  // row_bcast 15
+    x = dpp_max<0x143, 0xc>(x);  // row_bcast 31
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+// the exponent byte of a block from the bits of its largest magnitude (as integers, NaN > infinity > numbers)
+__device__ __forceinline__ uint32_t block_exponent(uint32_t top) {
+    const uint32_t e = (top + 0x0FFFFFu) >> 23;
+    return e < 1 ? 1 : e > 254 ? 255 : e;
+}
+constexpr int M_BIAS = 112, V_BIAS = 96;  // where the exponent field of the block's largest value lies: 127 - 15, 127 - 31
+
+__device__ __forceinline__ float decode_m(uint32_t code, uint32_t eb) {
+    const float x = ldexpf(__uint_as_float((code & 0x7F) << 20), (int)eb - 127 + M_BIAS);
+    const float y = eb == 255 ? __uint_as_float(0x7FC00000u) : x;
+    return __uint_as_float(__float_as_uint(y) | (code & 0x80) << 24);
+}
+__device__ __forceinline__ float decode_v(uint32_t code, uint32_t eb) {
+    const float x = ldexpf(__uint_as_float(code << 20), (int)eb - 127 + V_BIAS);
+    return eb == 255 ? __uint_as_float(0x7FC00000u) : x;
+}
+// noise: 16 random bits; they take the upper 16 of the 20 that are cut, the middle of what is below stands for the rest
+__device__ __forceinline__ uint32_t encode_m(float m, uint32_t eb, uint32_t noise) {
+    const uint32_t u = __float_as_uint(m);
+    const uint32_t y = __float_as_uint(ldexpf(__uint_as_float(u & 0x7FFFFFFFu), 127 - M_BIAS - (int)eb));
+    return eb == 255 ? 0 : ((y + (noise << 4 | 8)) >> 20) | (u >> 31) << 7;
+}
+__device__ __forceinline__ uint32_t encode_v(float v, uint32_t eb, uint32_t noise) {
+    const uint32_t y = __float_as_uint(ldexpf(fabsf(v), 127 - V_BIAS - (int)eb));
+    const uint32_t c = (y + (noise << 4 | 8)) >> 20;
+    return eb == 255 ? 0 : c == 0 && v > 0.f ? 1 : c;
+}
+// the four values of every lane of one block -> codes (byte j: value j) and the block's exponent byte; lanes past the end hold 0
+__device__ __forceinline__ uint32_t encode4_m(const float (&m)[4], const uint32_t (&h)[4], uint32_t& eb) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(m[j]) & 0x7FFFFFFFu);
+    eb = block_exponent(wave_max(top));
+    uint32_t c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c |= encode_m(m[j], eb, h[j] & 0xFFFF) << 8 * j;
+    return c;
+}
+__device__ __forceinline__ uint32_t encode4_v(const float (&v)[4], const uint32_t (&h)[4], uint32_t& eb) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    eb = block_exponent(wave_max(top));
+    uint32_t c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c |= encode_v(v[j], eb, h[j] >> 16) << 8 * j;
+    return c;
+}
+__device__ __forceinline__ void hash4(uint64_t at, const Scalars& s, uint32_t (&h)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = mix((uint32_t)(at + j), (uint32_t)((at + j) >> 32) * GOLDEN, s.k0, s.k1);
+}
+// stochastic rounding to bfloat16; infinities and NaN as they are
+__device__ __forceinline__ uint16_t round_bf16(float x, uint32_t h) {
+    const uint32_t u = __float_as_uint(x);
+    const bool finite = (u & 0x7F800000u) != 0x7F800000u;
+    const uint32_t r = finite ? u + ((h * GOLDEN) >> 16) : u | ((u & 0xFFFF) ? 0x400000u : 0);
+    return (uint16_t)(r >> 16);
+}
+
+__device__ __forceinline__ void update4(const Scalars& s, float factor, float (&p)[4], const float (&g)[4], float (&m)[4], float (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float gj = g[j] * factor;
+        m[j] = m[j] * s.b1 + gj * s.c1;
+        v[j] = v[j] * s.b2 + (gj * gj) * s.c2;
+        p[j] = p[j] * s.decay - (m[j] / (sqrtf(v[j]) * s.rbc2 + s.eps)) * s.step_size;
+    }
+}
+
+template <typename P, int BITS, bool FULL>
+__device__ __forceinline__ void step_piece(const Rec& r, const P* gp, const Scalars& s, float factor, int64_t off, int left, int lane) {
+    constexpr int GROUPS = PIECE / 256;
+    P* pp = (P*)r.p + off;
+    gp += off;
+    float p[GROUPS][4], g[GROUPS][4], m[GROUPS][4], v[GROUPS][4], e[GROUPS][4];
+    uint32_t mc[GROUPS], vc[GROUPS], meb[GROUPS], veb[GROUPS];
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+        if (!FULL && k * 256 >= left) break;
+        const int at = k * 256 + lane * 4, cnt = FULL ? 4 : left - at;
+        load4(pp + at, cnt, p[k]);
+        load4(gp + at, cnt, g[k]);
+        if (BITS == 32) {
+            load4((const float*)r.m + off + at, cnt, m[k]);
+            load4((const float*)r.v + off + at, cnt, v[k]);
+        } else {
+            mc[k] = load4b((const uint8_t*)r.m + off + at, cnt);
+            vc[k] = load4b((const uint8_t*)r.v + off + at, cnt);
+            meb[k] = r.me[off / QBLOCK + k];
+            veb[k] = r.ve[off / QBLOCK + k];
+        }
+        if (r.ema) load4(r.ema + off + at, cnt, e[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+        if (!FULL && k * 256 >= left) break;
+        const int at = k * 256 + lane * 4, cnt = FULL ? 4 : left - at;
+        if (BITS == 8) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                m[k][j] = decode_m(mc[k] >> 8 * j & 0xFF, meb[k]);
+                v[k][j] = decode_v(vc[k] >> 8 * j & 0xFF, veb[k]);
+            }
+        }
+        update4(s, factor, p[k], g[k], m[k], v[k]);
+        if (r.ema) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[k][j] = e[k][j] * s.d + p[k][j] * s.cd;
+            store4(r.ema + off + at, cnt, e[k]);
+        }
+        uint32_t h[4];
+        if (BITS == 8 || sizeof(P) == 2) hash4((uint64_t)(r.index + off + at), s, h);
+        if constexpr (sizeof(P) == 2) {
+            uint16_t q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[j] = round_bf16(p[k][j], h[j]);
+            store4(pp + at, cnt, q);
+        } else {
+            store4(pp + at, cnt, p[k]);
+        }
+        if (BITS == 32) {
+            store4((float*)r.m + off + at, cnt, m[k]);
+            store4((float*)r.v + off + at, cnt, v[k]);
+        } else {
+            if (!FULL) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {  // a lane past the end must not take part in the block's maximum
+                    m[k][j] = j < cnt ? m[k][j] : 0.f;
+                    v[k][j] = j < cnt ? v[k][j] : 0.f;
+                }
+            }
+            uint32_t eb;
+            const uint32_t a = encode4_m(m[k], h, eb);
+            if (lane == 0) r.me[off / QBLOCK + k] = (uint8_t)eb;
+            const uint32_t b = encode4_v(v[k], h, eb);
+            if (lane == 0) r.ve[off / QBLOCK + k] = (uint8_t)eb;
+            store4b((uint8_t*)r.m + off + at, cnt, a);
+            store4b((uint8_t*)r.v + off + at, cnt, b);
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t wave_number() {
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64));
+}
+
+template <typename P, int BITS>
+__global__ __launch_bounds__(256) void adamw_step_kernel(const Rec* __restrict__ recs, const Piece* __restrict__ pieces, uint32_t npieces,
+                                                         const void* const* __restrict__ grads, const float* __restrict__ factor_at,
+                                                         const Scalars* __restrict__ scalars_at, Scalars scalars) {
+    const uint32_t w = wave_number();
+    const int lane = threadIdx.x & 63;
+    if (w >= npieces) return;
+    const Piece c = pieces[w];
+    const void* gp = grads[c.tensor];
+    if (gp == (const void*)SR_ADAMW_SKIP) return;
+    const Rec r = recs[c.tensor];
+    if (!gp && !r.ema) return;
+    const Scalars s = scalars_at ? *scalars_at : scalars;
+    const float factor = factor_at ? *factor_at : 1.f;
+    const int64_t off = (int64_t)c.number * PIECE;
+    const int left = r.n - off < PIECE ? (int)(r.n - off) : PIECE;
+    if (!gp) {  // no gradient: the weights stay, their average goes on
+        for (int at = lane; at < left; at += 64) r.ema[off + at] = r.ema[off + at] * s.d + Elem<P>::ld((const P*)r.p + off + at) * s.cd;
+        return;
+    }
+    if (left == PIECE)
+        step_piece<P, BITS, true>(r, (const P*)gp, s, factor, off, left, lane);
+    else
+        step_piece<P, BITS, false>(r, (const P*)gp, s, factor, off, left, lane);
+}
+
+// step counter and scalars of a captured step: the host's values are fixed at capture, these move with every replay
+__global__ void adamw_tick_kernel(sr_adamw_hyper h, const float* lr, int64_t* step, Scalars* out) {
+    const int64_t t = *step + 1;
+    *step = t;
+    *out = make_scalars(h, lr ? (double)*lr : h.lr, t);
+}
+
+// moments as the values they stand for, at the tensors' places in one flat pair of arrays
+template <typename TO, int BITS>
+__global__ __launch_bounds__(256) void adamw_moments_kernel(const Rec* __restrict__ recs, const Piece* __restrict__ pieces, uint32_t npieces,
+                                                            TO* __restrict__ mo, TO* __restrict__ vo) {
+    const uint32_t w = wave_number();
+    const int lane = threadIdx.x & 63;
+    if (w >= npieces) return;
+    const Piece c = pieces[w];
+    const Rec r = recs[c.tensor];
+    const int64_t off = (int64_t)c.number * PIECE;
+    const int left = r.n - off < PIECE ? (int)(r.n - off) : PIECE;
+#pragma unroll
+    for (int k = 0; k < PIECE / 256; ++k) {
+        const int at = k * 256 + lane * 4, cnt = left - at;
+        if (cnt <= 0) return;
+        float m[4], v[4];
+        if (BITS == 32) {
+            load4((const float*)r.m + off + at, cnt, m);
+            load4((const float*)r.v + off + at, cnt, v);
+        } else {
+            const uint32_t a = load4b((const uint8_t*)r.m + off + at, cnt), b = load4b((const uint8_t*)r.v + off + at, cnt);
+            const uint32_t ea = r.me[off / QBLOCK + k], eb = r.ve[off / QBLOCK + k];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                m[j] = decode_m(a >> 8 * j & 0xFF, ea);
+                v[j] = decode_v(b >> 8 * j & 0xFF, eb);
+            }
+        }
+        if constexpr (sizeof(TO) == 2) {
+            uint16_t x[4], y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = f32_to_bf16(m[j]), y[j] = f32_to_bf16(v[j]);
+            store4(mo + r.index + off + at, cnt, x);
+            store4(vo + r.index + off + at, cnt, y);
+        } else {
+            store4(mo + r.index + off + at, cnt, m);
+            store4(vo + r.index + off + at, cnt, v);
+        }
+    }
+}
+
+template <int BITS>
+__global__ __launch_bounds__(256) void adamw_set_moments_kernel(const Rec* __restrict__ recs, const Piece* __restrict__ pieces, uint32_t npieces,
+                                                                const float* __restrict__ mi, const float* __restrict__ vi, Scalars s) {
+    const uint32_t w = wave_number();
+    const int lane = threadIdx.x & 63;
+    if (w >= npieces) return;
+    const Piece c = pieces[w];
+    const Rec r = recs[c.tensor];
+    const int64_t off = (int64_t)c.number * PIECE;
+    const int left = r.n - off < PIECE ? (int)(r.n - off) : PIECE;
+#pragma unroll
+    for (int k = 0; k < PIECE / 256; ++k) {
+        if (k * 256 >= left) return;
+        const int at = k * 256 + lane * 4, cnt = left - at;
+        float m[4], v[4];
+        load4(mi + r.index + off + at, cnt, m);
+        load4(vi + r.index + off + at, cnt, v);
+        if (BITS == 32) {
+            store4((float*)r.m + off + at, cnt, m);
+            store4((float*)r.v + off + at, cnt, v);
+        } else {
+            uint32_t h[4], eb;
+            hash4((uint64_t)(r.index + off + at), s, h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = v[j] >= 0.f ? v[j] : __uint_as_float(0x7FC00000u);  // no second moment: as sqrt has it
+            const uint32_t a = encode4_m(m, h, eb);
+            if (lane == 0) r.me[off / QBLOCK + k] = (uint8_t)eb;
+            const uint32_t b = encode4_v(v, h, eb);
+            if (lane == 0) r.ve[off / QBLOCK + k] = (uint8_t)eb;
+            store4b((uint8_t*)r.m + off + at, cnt, a);
+            store4b((uint8_t*)r.v + off + at, cnt, b);
+        }
+    }
+}
+
+// ---- global gradient norm ---------------------------------------------------------------------------------------------
+// Squares are added in float64 (a float32 square overflows from 1.8e19 on, and 1e8 of them lose three digits), in an order
+// that the shapes alone determine.  Work items are runs of consecutive values; waves take them in turn.
+struct PieceSource {  // the pieces of an optimizer's list, gradients by tensor
+    const Rec* recs;
+    const Piece* pieces;
+    const void* const* grads;
+    template <typename T>
+    __device__ __forceinline__ const T* run(uint32_t i, int64_t& n) const {
+        const Piece c = pieces[i];
+        const T* g = (const T*)grads[c.tensor];
+        n = 0;
+        if (!g || g == (const T*)SR_ADAMW_SKIP) return g;
+        const int64_t off = (int64_t)c.number * PIECE, left = recs[c.tensor].n - off;
+        n = left < PIECE ? left : PIECE;
+        return g + off;
+    }
+};
+struct SpanSource {
+    const sr_grad_span* spans;
+    template <typename T>
+    __device__ __forceinline__ const T* run(uint32_t i, int64_t& n) const {
+        n = spans[i].n;
+        return (const T*)spans[i].g;
+    }
+};
+
+__device__ __forceinline__ double wave_sum(double x) {
+#pragma unroll
+    for (int k = 32; k; k >>= 1) x += __shfl_xor(x, k, 64);
+    return x;
+}
+
+template <typename T, typename S>
+__global__ __launch_bounds__(256) void grad_norm_kernel(S src, uint32_t items, double* __restrict__ partial) {
+    __shared__ double sums[4];
+    const int lane = threadIdx.x & 63;
+    double acc[4] = {0, 0, 0, 0};
+    for (uint32_t i = wave_number(); i < items; i += gridDim.x * 4) {
+        int64_t n;
+        const T* g = src.template run<T>(i, n);
+        int64_t at = lane * 4;
+        for (; at + 3 * 256 + 4 <= n; at += 1024) {
+            float x[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) load4(g + at + k * 256, 4, x[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j] = fma((double)x[k][j], (double)x[k][j], acc[j]);
+        }
+        for (; at < n; at += 256) {
+            float x[4];
+            load4(g + at, n - at < 4 ? (int)(n - at) : 4, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j] = fma((double)x[j], (double)x[j], acc[j]);
+        }
+    }
+    const double sum = wave_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
+    if (lane == 0) sums[threadIdx.x / 64] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) partial[blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+}
+
+struct Partials {
+    int32_t n[SR_GRAD_MAX_LISTS];
+    int32_t lists;
+};
+__global__ __launch_bounds__(256) void grad_norm_finish_kernel(Partials parts, const double* __restrict__ partial, double max_norm, float* __restrict__ out) {
+    __shared__ double sums[4];
+    double acc = 0;
+    for (int l = 0; l < parts.lists; ++l)
+        for (int i = threadIdx.x; i < parts.n[l]; i += 256) acc += partial[l * NORM_WG + i];
+    acc = wave_sum(acc);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x / 64] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const double norm = sqrt((sums[0] + sums[1]) + (sums[2] + sums[3]));
+        const double f = max_norm / (norm + 1e-6);
+        out[0] = (float)norm;
+        out[1] = f >= 1.0 ? 1.f : (float)f;  // NaN stays
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void grad_scale_kernel(const sr_grad_span* __restrict__ spans, uint32_t items, const float* __restrict__ factor_at) {
+    const float factor = *factor_at;
+    if (factor == 1.f) return;
+    const int lane = threadIdx.x & 63;
+    for (uint32_t i = wave_number(); i < items; i += gridDim.x * 4) {
+        T* g = (T*)spans[i].g;
+        const int64_t n = spans[i].n;
+        for (int64_t at = lane * 4; at < n; at += 256) {
+            const int cnt = n - at < 4 ? (int)(n - at) : 4;
+            float x[4];
+            load4(g + at, cnt, x);
+            if constexpr (sizeof(T) == 2) {
+                uint16_t y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = f32_to_bf16(x[j] * factor);
+                store4(g + at, cnt, y);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] *= factor;
+                store4(g + at, cnt, x);
+            }
+        }
+    }
+}
+
+// ---- small host -> device copies through kernel arguments ---------------------------------------------------------------
+constexpr int UPLOAD = 3840;  // bytes per launch: kernel arguments are 4 KB
+struct UploadArgs {
+    uint64_t dst;
+    int32_t bytes;
+    int32_t pad;
+    uint32_t data[UPLOAD / 4];
+};
+__global__ __launch_bounds__(256) void upload_kernel(UploadArgs a) {
+    for (int i = threadIdx.x; i < a.bytes / 4; i += 256) ((uint32_t*)a.dst)[i] = a.data[i];
+}
+
+}  // namespace sr
+
+using namespace sr;
+
+struct sr_adamw {
+    int dtype, bits, count, device;
+    uint32_t npieces;
+    bool ema;
+    void* tables;  // Rec[count], Piece[npieces]
+    const Rec* recs() const { return (const Rec*)tables; }
+    const Piece* pieces() const { return (const Piece*)((const char*)tables + sizeof(Rec) * (size_t)count); }
+};
+
+namespace {
+int build_tables(const sr_adamw_tensor* t, int count, int dtype, int bits, std::vector<Rec>& recs, std::vector<Piece>& pieces, bool& ema) {
+    int with_ema = 0;
+    uint64_t total = 0;
+    for (int i = 0; i < count; ++i) {
+        const sr_adamw_tensor& x = t[i];
+        SR_REQUIRE(x.n >= 0 && x.n <= ((int64_t)1 << 40) && x.index >= 0 && x.index <= ((int64_t)1 << 50));
+        SR_REQUIRE(x.n == 0 || (x.p && x.m && x.v && (bits == 32 || (x.me && x.ve))));
+        const uintptr_t align = dtype == SR_F32 ? 4 : 2;
+        SR_REQUIRE((uintptr_t)x.p % align == 0 && (uintptr_t)x.ema % 4 == 0);
+        SR_REQUIRE(bits == 8 || ((uintptr_t)x.m % 4 == 0 && (uintptr_t)x.v % 4 == 0));
+        if (x.n) with_ema |= x.ema ? 1 : 2;
+        total += (uint64_t)(x.n + PIECE - 1) / PIECE;
+    }
+    SR_REQUIRE(with_ema != 3 && total <= 0x7FFFFFFFu);
+    ema = with_ema == 1;
+    recs.resize(count);
+    pieces.reserve(total);
+    for (int i = 0; i < count; ++i) {
+        recs[i] = {t[i].p, t[i].m, t[i].v, t[i].me, t[i].ve, t[i].ema, t[i].n, t[i].index};
+        const uint32_t k = (uint32_t)((t[i].n + PIECE - 1) / PIECE);
+        for (uint32_t j = 0; j < k; ++j) pieces.push_back({(uint32_t)i, j});
+    }
+    return SR_OK;
+}
+int on_device(const sr_adamw* l) {
+    int dev = 0;
+    SR_HIP(hipGetDevice(&dev));
+    return dev == l->device ? SR_OK : SR_ERR_STATE;
+}
+uint32_t waves_to_wgs(uint32_t waves) { return (waves + 3) / 4; }
+int check_hyper(const sr_adamw_hyper* h, int64_t step) {
+    SR_REQUIRE(h);
+    SR_REQUIRE(h->lr >= 0 && h->beta1 >= 0 && h->beta1 < 1 && h->beta2 >= 0 && h->beta2 < 1 && h->eps >= 0 && h->weight_decay >= 0);
+    SR_REQUIRE(h->ema_decay >= 0 && h->ema_decay <= 1 && step >= 1);
+    return SR_OK;
+}
+}  // namespace
+
+extern "C" int sr_adamw_create(int dtype, int bits, int count, const sr_adamw_tensor* tensors, sr_adamw** out) {
+    SR_REQUIRE(out && count > 0 && tensors && (dtype == SR_F32 || dtype == SR_BF16) && (bits == 32 || bits == 8));
+    *out = nullptr;
+    try {
+        std::vector<Rec> recs;
+        std::vector<Piece> pieces;
+        bool ema = false;
+        const int rc = build_tables(tensors, count, dtype, bits, recs, pieces, ema);
+        if (rc) return rc;
+        int dev = 0;
+        SR_HIP(hipGetDevice(&dev));
+        sr_adamw* l = new sr_adamw{dtype, bits, count, dev, (uint32_t)pieces.size(), ema, nullptr};
+        const size_t rb = sizeof(Rec) * recs.size(), pb = sizeof(Piece) * pieces.size();
+        hipError_t e = hipMalloc(&l->tables, rb + pb);
+        if (e == hipSuccess) e = hipMemcpy(l->tables, recs.data(), rb, hipMemcpyHostToDevice);
+        if (e == hipSuccess && pb) e = hipMemcpy((char*)l->tables + rb, pieces.data(), pb, hipMemcpyHostToDevice);
+        if (e != hipSuccess) {
+            sr_adamw_destroy(l);
+            return hip_fail(e);
+        }
+        *out = l;
+        return SR_OK;
+    } catch (...) {  // no memory for the tables
+        return SR_ERR_STATE;
+    }
+}
+
+extern "C" void sr_adamw_destroy(sr_adamw* l) {
+    if (!l) return;
+    if (l->tables) (void)hipFree(l->tables);
+    delete l;
+}
+
+extern "C" int sr_adamw_step(const sr_adamw* l, const sr_adamw_hyper* h, int64_t step, const void* scalars, const void* const* grads,
+                             const float* factor, void* stream) {
+    SR_REQUIRE(l && grads);
+    Scalars s = {};
+    if (!scalars) {
+        const int rc = check_hyper(h, step);
+        if (rc) return rc;
+        s = make_scalars(*h, h->lr, step);
+    }
+    const int rc = on_device(l);
+    if (rc) return rc;
+    if (!l->npieces) return SR_OK;
+    const dim3 grid(waves_to_wgs(l->npieces));
+    hipStream_t st = (hipStream_t)stream;
+    const Scalars* at = (const Scalars*)scalars;
+#define SR_STEP(P, BITS) adamw_step_kernel<P, BITS><<<grid, 256, 0, st>>>(l->recs(), l->pieces(), l->npieces, grads, factor, at, s)
+    if (l->dtype == SR_F32) {
+        if (l->bits == 32)
+            SR_STEP(float, 32);
+        else
+            SR_STEP(float, 8);
+    } else {
+        if (l->bits == 32)
+            SR_STEP(bf16_t, 32);
+        else
+            SR_STEP(bf16_t, 8);
+    }
+#undef SR_STEP
+    SR_LAUNCH_CHECK();
+    return SR_OK;
+}
+
+extern "C" int sr_adamw_tick(const sr_adamw_hyper* h, const float* lr, int64_t* step, void* scalars, void* stream) {
+    SR_REQUIRE(step && scalars);
+    static_assert(sizeof(Scalars) <= SR_ADAMW_SCALARS_BYTES, "size in the header");
+    const int rc = check_hyper(h, 1);
+    if (rc) return rc;
+    adamw_tick_kernel<<<1, 1, 0, (hipStream_t)stream>>>(*h, lr, step, (Scalars*)scalars);
+    SR_LAUNCH_CHECK();
+    return SR_OK;
+}
+
+extern "C" int sr_adamw_moments(const sr_adamw* l, int dtype, void* m, void* v, void* stream) {
+    SR_REQUIRE(l && m && v && (dtype == SR_F32 || dtype == SR_BF16));
+    const int rc = on_device(l);
+    if (rc) return rc;
+    if (!l->npieces) return SR_OK;
+    const dim3 grid(waves_to_wgs(l->npieces));
+    hipStream_t st = (hipStream_t)stream;
+#define SR_MOMENTS(T, BITS) adamw_moments_kernel<T, BITS><<<grid, 256, 0, st>>>(l->recs(), l->pieces(), l->npieces, (T*)m, (T*)v)
+    if (dtype == SR_F32) {
+        if (l->bits == 32)
+            SR_MOMENTS(float, 32);
+        else
+            SR_MOMENTS(float, 8);
+    } else {
+        if (l->bits == 32)
+            SR_MOMENTS(bf16_t, 32);
+        else
+            SR_MOMENTS(bf16_t, 8);
+    }
+#undef SR_MOMENTS
+    SR_LAUNCH_CHECK();
+    return SR_OK;
+}
+
+extern "C" int sr_adamw_set_moments(const sr_adamw* l, const float* m, const float* v, uint64_t seed, void* stream) {
+    SR_REQUIRE(l && m && v);
+    const int rc = on_device(l);
+    if (rc) return rc;
+    if (!l->npieces) return SR_OK;
+    Scalars s = {};
+    make_key(seed, 0, s);
+    const dim3 grid(waves_to_wgs(l->npieces));
+    if (l->bits == 32)
+        adamw_set_moments_kernel<32><<<grid, 256, 0, (hipStream_t)stream>>>(l->recs(), l->pieces(), l->npieces, m, v, s);
+    else
+        adamw_set_moments_kernel<8><<<grid, 256, 0, (hipStream_t)stream>>>(l->recs(), l->pieces(), l->npieces, m, v, s);
+    SR_LAUNCH_CHECK();
+    return SR_OK;
+}
+
+extern "C" size_t sr_grad_norm_workspace_bytes(int nlists) { return nlists > 0 ? (size_t)nlists * NORM_WG * sizeof(double) : 0; }
+
+extern "C" int sr_grad_norm(int nlists, const sr_grad_list* lists, double max_norm, float* out, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+    SR_REQUIRE(nlists >= 0 && nlists <= SR_GRAD_MAX_LISTS && (lists || !nlists) && out && max_norm >= 0);
+    for (int i = 0; i < nlists; ++i) {
+        const sr_grad_list& l = lists[i];
+        if (l.list) {
+            SR_REQUIRE(l.grads);
+            const int rc = on_device(l.list);
+            if (rc) return rc;
+        } else {
+            SR_REQUIRE((l.dtype == SR_F32 || l.dtype == SR_BF16) && l.nspans >= 0 && l.nspans <= 0x7FFFFFFF && (l.spans || !l.nspans));
+        }
+    }
+    if (nlists && (!workspace || workspace_bytes < sr_grad_norm_workspace_bytes(nlists))) return SR_ERR_WORKSPACE;
+    SR_REQUIRE((uintptr_t)workspace % 8 == 0);
+    hipStream_t st = (hipStream_t)stream;
+    Partials parts = {};
+    parts.lists = nlists;
+    for (int i = 0; i < nlists; ++i) {
+        const sr_grad_list& l = lists[i];
+        const uint32_t items = l.list ? l.list->npieces : (uint32_t)l.nspans;
+        if (!items) continue;
+        const uint32_t want = waves_to_wgs(items), wgs = want < NORM_WG ? want : NORM_WG;
+        parts.n[i] = (int32_t)wgs;
+        double* out_i = (double*)workspace + (size_t)i * NORM_WG;
+        const int dtype = l.list ? l.list->dtype : l.dtype;
+        if (l.list) {
+            const PieceSource src = {l.list->recs(), l.list->pieces(), l.grads};
+            if (dtype == SR_F32)
+                grad_norm_kernel<float><<<wgs, 256, 0, st>>>(src, items, out_i);
+            else
+                grad_norm_kernel<bf16_t><<<wgs, 256, 0, st>>>(src, items, out_i);
+        } else {
+            const SpanSource src = {l.spans};
+            if (dtype == SR_F32)
+                grad_norm_kernel<float><<<wgs, 256, 0, st>>>(src, items, out_i);
+            else
+                grad_norm_kernel<bf16_t><<<wgs, 256, 0, st>>>(src, items, out_i);
+        }
+        SR_LAUNCH_CHECK();
+    }
+    grad_norm_finish_kernel<<<1, 256, 0, st>>>(parts, (const double*)workspace, max_norm, out);
+    SR_LAUNCH_CHECK();
+    return SR_OK;
+}
+
+extern "C" int sr_grad_scale(int dtype, int64_t nspans, const sr_grad_span* spans, const float* factor, void* stream) {
+    SR_REQUIRE((dtype == SR_F32 || dtype == SR_BF16) && nspans >= 0 && nspans <= 0x7FFFFFFF && (spans || !nspans) && factor);
+    if (!nspans) return SR_OK;
+    const uint32_t want = waves_to_wgs((uint32_t)nspans), wgs = want < NORM_WG ? want : NORM_WG;
+    if (dtype == SR_F32)
+        grad_scale_kernel<float><<<wgs, 256, 0, (hipStream_t)stream>>>(spans, (uint32_t)nspans, factor);
+    else
+        grad_scale_kernel<bf16_t><<<wgs, 256, 0, (hipStream_t)stream>>>(spans, (uint32_t)nspans, factor);
+    SR_LAUNCH_CHECK();
+    return SR_OK;
+}
+
+extern "C" int sr_upload(const void* src_host, void* dst, size_t bytes, void* stream) {
+    SR_REQUIRE(bytes % 4 == 0 && (uintptr_t)dst % 4 == 0 && ((src_host && dst) || !bytes));
+    for (size_t at = 0; at < bytes; at += UPLOAD) {
+        UploadArgs a;
+        a.dst = (uint64_t)(uintptr_t)dst + at;
+        a.bytes = (int32_t)(bytes - at < UPLOAD ? bytes - at : UPLOAD);
+        a.pad = 0;
+        memcpy(a.data, (const char*)src_host + at, a.bytes);
+        upload_kernel<<<1, 256, 0, (hipStream_t)stream>>>(a);
+        SR_LAUNCH_CHECK();
+    }
+    return SR_OK;
+}

@@ -1,0 +1,188 @@
+// Host side of the optimizers: reads the gradients of thousands of parameters in one call.
+//
+// A training step of RRDBNet-FDConv has 8380 parameter tensors whose `.grad` are new tensors every step.  Reading 8380 data
+// pointers and checking dtype, device and layout takes Python 4 ms, the same walk over the tensors' C++ objects 0.3 ms -- and the
+// kernels that then run take 0.1.  Built as libsr_amd_torch.so (the only file that sees torch's C++ headers); Python calls it
+// through ctypes with the GIL held.  No exception leaves a function: they return SRT_FAILED and keep the message.
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
+#include <cstring>
+#include <string>
+#include <vector>
+
+#define SRT_FAILED (-1)
+#define SRT_API extern "C" __attribute__((visibility("default")))
+
+namespace {
+thread_local std::string g_message;
+
+template <typename F>
+int64_t guarded(F f) {
+    try {
+        return f();
+    } catch (const std::exception& e) {
+        g_message = e.what();
+    } catch (...) {
+        g_message = "unknown C++ exception";
+    }
+    return SRT_FAILED;
+}
+
+const at::Tensor& tensor_of(PyObject* o) {
+    TORCH_CHECK(THPVariable_Check(o), "not a tensor");
+    return THPVariable_Unpack(o);
+}
+
+struct Tracked {
+    std::vector<at::Tensor> params;
+    struct Was {
+        const void* data;
+        int64_t numel;
+        caffe2::TypeMeta dtype;
+        c10::Device device;
+    };
+    std::vector<Was> was;
+};
+
+struct Span {
+    uint64_t g;
+    int64_t n;
+};
+std::vector<Span> g_spans[2];  // what the last srt_spans found: float32, bfloat16 (guarded by the GIL)
+
+// the same memory order: element i of one is element i of the other
+bool same_layout(const c10::TensorImpl* a, const c10::TensorImpl* b) {
+    return (a->is_contiguous() && b->is_contiguous()) || (a->strides().equals(b->strides()) && a->is_non_overlapping_and_dense());
+}
+}  // namespace
+
+SRT_API const char* srt_message() { return g_message.c_str(); }
+
+// holds the tensors of a list (they stay alive); NULL on failure
+SRT_API void* srt_track(PyObject* list) {
+    Tracked* t = nullptr;
+    const int64_t rc = guarded([&]() -> int64_t {
+        TORCH_CHECK(PyList_Check(list), "not a list");
+        t = new Tracked;
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+            const at::Tensor& p = tensor_of(PyList_GET_ITEM(list, i));
+            t->params.push_back(p);
+            const c10::TensorImpl* impl = p.unsafeGetTensorImpl();
+            t->was.push_back({impl->data(), impl->numel(), impl->dtype(), impl->device()});
+        }
+        return 0;
+    });
+    if (rc) {
+        delete t;
+        return nullptr;
+    }
+    return t;
+}
+SRT_API void srt_untrack(void* h) { delete (Tracked*)h; }
+
+// out[i] = address of the gradient of tensor i, 0 without one.  Returns the number of tensors without a gradient.
+// odd[0 .. *nodd): tensors whose gradient cannot be read as it lies (other shape, strides, dtype or device: out[i] = 0, not counted
+// as missing).  *moved: tensors that are not where, or what, they were when the list was made.
+SRT_API int64_t srt_gradients(void* h, uint64_t* out, int64_t* odd, int64_t* nodd, int64_t* moved) {
+    return guarded([&]() -> int64_t {
+        const Tracked& t = *(const Tracked*)h;
+        const size_t n = t.params.size();
+        int64_t missing = 0;
+        *nodd = *moved = 0;
+        for (size_t i = 0; i < n; ++i) {
+            c10::TensorImpl* p = t.params[i].unsafeGetTensorImpl();
+            const Tracked::Was& was = t.was[i];
+            if (p->data() != was.data || p->numel() != was.numel || p->dtype() != was.dtype || p->device() != was.device) ++*moved;
+            const at::Tensor& grad = static_cast<const c10::TensorImpl*>(p)->grad();
+            out[i] = 0;
+            if (!grad.defined()) {
+                ++missing;
+                continue;
+            }
+            const c10::TensorImpl* g = grad.unsafeGetTensorImpl();
+            if (g->layout() == at::kStrided && g->numel() == p->numel() && g->dtype() == p->dtype() && g->device() == p->device() && same_layout(g, p))
+                out[i] = (uint64_t)(uintptr_t)g->data();
+            else
+                odd[(*nodd)++] = (int64_t)i;
+        }
+        return missing;
+    });
+}
+
+// the tensors were written in place (autograd's saved-tensor checks and caches keyed on the version must see it);
+// skip != NULL: only where skip[i] != 0
+SRT_API int64_t srt_written(void* h, const uint64_t* skip) {
+    return guarded([&]() -> int64_t {
+        const Tracked& t = *(const Tracked*)h;
+        for (size_t i = 0; i < t.params.size(); ++i)
+            if (!skip || skip[i]) t.params[i].unsafeGetTensorImpl()->bump_version();
+        return 0;
+    });
+}
+
+// The gradients of a list of parameters (of_params) or of a list of gradients, as spans of consecutive values of at most
+// `longest` (0: by the total, see below); counts[0 / 1]: spans in float32 / bfloat16, counts[2]: tensors.  Returns 0, or
+//   1 + i: tensor i is neither float32 nor bfloat16, or not on GPU `device` (device < 0: that of the first, put into *device)
+//   -2 - i: gradient i has holes or repeats its elements
+// and SRT_FAILED.  Gradients that share memory fail: they would be scaled twice.
+SRT_API int64_t srt_spans(PyObject* list, int of_params, int* device, int64_t* counts) {
+    return guarded([&]() -> int64_t {
+        TORCH_CHECK(PyList_Check(list), "not a list");
+        std::vector<Span> found[2];
+        g_spans[0].clear();
+        g_spans[1].clear();
+        counts[0] = counts[1] = counts[2] = 0;
+        int64_t total = 0;
+        uint64_t last = 0;
+        bool ascending = true;
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+            const at::Tensor& x = tensor_of(PyList_GET_ITEM(list, i));
+            c10::TensorImpl* g = x.unsafeGetTensorImpl();
+            if (of_params) {
+                const at::Tensor& grad = static_cast<const c10::TensorImpl*>(g)->grad();
+                if (!grad.defined()) continue;
+                g = grad.unsafeGetTensorImpl();
+            }
+            ++counts[2];
+            if (!g->is_inference()) g->bump_version();  // they are about to be written
+            if (g->layout() != at::kStrided || !g->device().is_cuda()) return 1 + i;
+            if (*device < 0) *device = g->device().index();
+            const int kind = g->dtype() == caffe2::TypeMeta::Make<float>() ? 0 : g->dtype() == caffe2::TypeMeta::Make<at::BFloat16>() ? 1 : -1;
+            if (kind < 0 || g->device().index() != *device) return 1 + i;
+            if (!g->is_contiguous() && !g->is_non_overlapping_and_dense()) return -2 - i;
+            const int64_t n = g->numel();
+            if (!n) continue;
+            const uint64_t at = (uint64_t)(uintptr_t)g->data();
+            ascending &= at >= last;
+            last = at + (uint64_t)n * (kind ? 2 : 4);
+            found[kind].push_back({at, n});
+            total += n;
+        }
+        if (!ascending) {
+            std::vector<std::pair<uint64_t, uint64_t>> all;
+            for (int k = 0; k < 2; ++k)
+                for (const Span& s : found[k]) all.emplace_back(s.g, s.g + (uint64_t)s.n * (k ? 2 : 4));
+            std::sort(all.begin(), all.end());
+            for (size_t i = 1; i < all.size(); ++i) TORCH_CHECK(all[i].first >= all[i - 1].second, "two gradients share memory");
+        }
+        // a wave takes a span at a time and 8192 waves run at once: equal shares of long tensors, none below 4096 values
+        const int64_t longest = std::max<int64_t>(4096, (total / 8192 + 1023) / 1024 * 1024);
+        for (int k = 0; k < 2; ++k) {
+            for (const Span& s : found[k])
+                for (int64_t at = 0; at < s.n; at += longest)
+                    g_spans[k].push_back({s.g + (uint64_t)at * (k ? 2 : 4), std::min(longest, s.n - at)});
+            counts[k] = (int64_t)g_spans[k].size();
+        }
+        return 0;
+    });
+}
+// copies them out: float32 first
+SRT_API void srt_take_spans(void* dst) {
+    char* to = (char*)dst;
+    for (int k = 0; k < 2; ++k) {
+        if (!g_spans[k].empty()) memcpy(to, g_spans[k].data(), g_spans[k].size() * sizeof(Span));
+        to += g_spans[k].size() * sizeof(Span);
+        g_spans[k].clear();
+    }
+}

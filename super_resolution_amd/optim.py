@@ -1,0 +1,587 @@
+"""AdamW over many tensors, with moments in 32 or in 8 bits, and clipping by the global gradient norm, on libsr_amd.
+
+Reference: `torch.optim.Adam(...)` / `optimizer.step()` of train/train_realESRGAN_fdconv_1.py:104,118, `clip_grad_norm_(..., 1.0)` of
+train/train_realESRGAN_fdconv.py:142, and the weight average that Real-ESRGAN checkpoints carry as `params_ema`
+(Real-ESRGAN-master/realesrgan/utils.py:59-63).
+
+`train.FlatAdam` re-points the parameters into one buffer and runs torch operators on it; `AdamW` leaves them where they are:
+one kernel (csrc/adamw.hip) walks all tensors of a group, reads gradients, parameters and moments once and writes them once.
+"""
+import ctypes as C
+import os
+
+import numpy as np
+import torch
+
+from . import _lib as L
+
+_HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libsr_amd_torch.so')
+_host = None
+_BY_VALUE = 4 * 3840   # bytes of a table that go to the device as kernel arguments (four launches); longer ones are copied
+
+
+def _host_lib():
+    """libsr_amd_torch.so (csrc/torch_host.cpp): reads torch's tensor objects, with the GIL held."""
+    global _host
+    if _host is None:
+        if not os.path.exists(_HOST_PATH):
+            raise RuntimeError('%s is missing: build it with `python -m super_resolution_amd.build`; there is no fallback path' % _HOST_PATH)
+        h = C.PyDLL(_HOST_PATH)
+        h.srt_message.restype, h.srt_message.argtypes = C.c_char_p, []
+        h.srt_track.restype, h.srt_track.argtypes = C.c_void_p, [C.py_object]
+        h.srt_untrack.restype, h.srt_untrack.argtypes = None, [C.c_void_p]
+        h.srt_gradients.restype, h.srt_gradients.argtypes = C.c_int64, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+        h.srt_written.restype, h.srt_written.argtypes = C.c_int64, [C.c_void_p, C.c_void_p]
+        h.srt_spans.restype, h.srt_spans.argtypes = C.c_int64, [C.py_object, C.c_int, C.c_void_p, C.c_void_p]
+        h.srt_take_spans.restype, h.srt_take_spans.argtypes = None, [C.c_void_p]
+        _host = h
+    return _host
+
+
+def _host_failed(what):
+    raise RuntimeError('%s: %s' % (what, _host_lib().srt_message().decode()))
+
+
+def _upload(nbytes, write, dev):
+    """A table of nbytes on the device; write(address) fills it on the host.  Under capture it travels by value: a copy node would
+    read the host buffer again at every replay."""
+    table = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+    if nbytes <= _BY_VALUE or torch.cuda.is_current_stream_capturing():
+        buf = (C.c_char * max(nbytes, 1))()
+        write(C.addressof(buf))
+        L.check(L.lib().sr_upload(C.addressof(buf), table.data_ptr(), nbytes, L.stream_ptr(dev)), 'sr_upload')
+    else:
+        stage = torch.empty(nbytes, dtype=torch.uint8, pin_memory=True)
+        write(stage.data_ptr())
+        table.copy_(stage, non_blocking=True)   # torch keeps the pinned block until the copy is done
+    return table
+
+
+def _exchange_gradients(params, group, average):
+    """Gradients summed (or averaged) over the ranks; `group`: the ProcessGroup."""
+    import torch.distributed as dist
+    from .train import allreduce_gradients
+    grads = [p for p in params if p.requires_grad]
+    if not (grads and grads[0].is_cuda and dist.get_backend(group) == 'gloo'):
+        allreduce_gradients(grads, group=group, average=average)
+        return
+    # gloo reduces host memory (its device path stalls when ranks share one GPU)
+    for dt in sorted({p.dtype for p in grads}, key=str):
+        part = [p for p in grads if p.dtype == dt]
+        host = torch.cat([(p.grad if p.grad is not None else torch.zeros_like(p)).reshape(-1) for p in part]).cpu()
+        dist.all_reduce(host, op=dist.ReduceOp.SUM, group=group)
+        if average:
+            host /= dist.get_world_size(group)
+        flat = host.to(part[0].device)
+        for p, g in zip(part, flat.split([p.numel() for p in part])):
+            p.grad = g.view(p.shape).clone() if p.grad is None else p.grad.copy_(g.view(p.shape))
+
+
+def _broadcast_parameters(params, group):
+    """Rank 0's values everywhere, one collective per dtype."""
+    import torch.distributed as dist
+    src = dist.get_global_rank(group, 0) if group is not None else 0
+    for dt in sorted({p.dtype for p in params}, key=str):
+        part = [p for p in params if p.dtype == dt]
+        flat = torch.cat([p.reshape(-1) for p in part])
+        if flat.is_cuda and dist.get_backend(group) == 'gloo':
+            host = flat.cpu()
+            dist.broadcast(host, src=src, group=group)
+            flat.copy_(host)
+        else:
+            dist.broadcast(flat, src=src, group=group)
+        for p, x in zip(part, flat.split([p.numel() for p in part])):
+            p.copy_(x.view(p.shape))
+
+
+def _world(group):
+    import torch.distributed as dist
+    return dist.get_world_size(group) if dist.is_available() and dist.is_initialized() else 1
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# clipping
+# ------------------------------------------------------------------------------------------------------------------
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ (2-norm): scales the gradients in place by min(1, max_norm / (norm + 1e-6)) and returns the
+    norm, a 0-d float32 tensor.  Squares are summed in float64, in an order that the shapes alone determine; nothing waits for
+    the GPU unless error_if_nonfinite is set.  float32 and bfloat16 gradients, mixed, on one GPU."""
+    params = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError('clip_grad_norm_: max_norm must not be negative (got %r)' % max_norm)
+    host, lib = _host_lib(), L.lib()
+    device, counts = C.c_int(-1), (C.c_int64 * 3)()
+    rc = host.srt_spans(params, 1, C.byref(device), counts)
+    odd = []
+    if rc <= -2:   # gradients with holes (or expanded ones): the norm reads dense copies, torch scales the originals
+        grads = [p.grad for p in params if p.grad is not None]
+        dense = []
+        for g in grads:
+            c = g if _is_dense(g) else g.contiguous()
+            if c is not g:
+                odd.append(g)
+            dense.append(c)
+        device = C.c_int(-1)
+        rc = host.srt_spans(dense, 0, C.byref(device), counts)
+    if rc == -1:
+        _host_failed('clip_grad_norm_')
+    if rc > 0:
+        raise TypeError('clip_grad_norm_: gradients are float32 or bfloat16 on one GPU; tensor %d is not' % (rc - 1))
+    if not counts[2]:
+        return torch.tensor(0.0)
+    dev = torch.device('cuda', device.value)
+    with torch.cuda.device(dev):
+        n32, n16 = counts[0], counts[1]
+        spans = _upload(16 * (n32 + n16), host.srt_take_spans, dev)
+        lists = (L.GradList * 2)()
+        lists[0].spans, lists[0].nspans, lists[0].dtype = spans.data_ptr(), n32, L.SR_F32
+        lists[1].spans, lists[1].nspans, lists[1].dtype = spans.data_ptr() + 16 * n32, n16, L.SR_BF16
+        out = _norm(lists, max_norm, dev)
+        if error_if_nonfinite and not bool(torch.isfinite(out[0])):
+            raise RuntimeError('clip_grad_norm_: the norm of the gradients is not finite')
+        factor, st = out.data_ptr() + 4, L.stream_ptr(dev)
+        for l in lists:
+            if l.nspans:
+                L.check(lib.sr_grad_scale(l.dtype, l.nspans, l.spans, factor, st), 'sr_grad_scale')
+        for g in odd:
+            g.mul_(out[1])
+    return out[0]
+
+
+def _is_dense(t):
+    """Whether the tensor's elements fill one run of memory, each once."""
+    if t.is_contiguous():
+        return True
+    n = 1
+    for size, stride in sorted(((s, st) for s, st in zip(t.shape, t.stride()) if s != 1), key=lambda x: x[1]):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def _norm(lists, max_norm, dev):
+    """(norm, factor) as a float32 pair on the device."""
+    lib, n = L.lib(), len(lists)
+    out = torch.empty(2, dtype=torch.float32, device=dev)
+    ws = torch.empty(lib.sr_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
+    L.check(lib.sr_grad_norm(n, lists, max_norm, out.data_ptr(), ws.data_ptr(), ws.numel(), L.stream_ptr(dev)), 'sr_grad_norm')
+    return out
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# AdamW
+# ------------------------------------------------------------------------------------------------------------------
+class _List:
+    """The tensors of one parameter group with one dtype: the device tables, and the walk over their gradients."""
+
+    def __init__(self, opt, group, bits, members):
+        self.group, self.bits, self.members = group, bits, members   # members: indices into opt.params
+        self.params = [opt.params[i] for i in members]
+        self.n = len(members)
+        self.sizes = [p.numel() for p in self.params]
+        self.dtype = self.params[0].dtype
+        self.handle, self.tracked, self.retired = None, None, []
+        self.steps = 0              # int: all tensors alike; else an int64 array
+        self.ptrs = (C.c_uint64 * self.n)()
+        self.odd = (C.c_int64 * self.n)()
+        self.nodd, self.moved = C.c_int64(), C.c_int64()
+        self.seen = self.step_dev = self.scalars = None
+        if opt.capturable:          # fixed memory: captured graphs point to it
+            self.step_dev = torch.zeros((), dtype=torch.int64, device=opt.device)
+            self.scalars = torch.empty(L.ADAMW_SCALARS_BYTES, dtype=torch.uint8, device=opt.device)
+
+    def build(self, opt):
+        arr = (L.AdamWTensor * self.n)()
+        for t, i, p in zip(arr, self.members, self.params):
+            t.p, t.n, t.index = p.data_ptr(), p.numel(), opt._index[i]
+            if self.bits == 32:
+                t.m = opt._m32.data_ptr() + 4 * opt._at[i]
+                t.v = opt._v32.data_ptr() + 4 * opt._at[i]
+            else:
+                t.m, t.v = opt._m8.data_ptr() + opt._at[i], opt._v8.data_ptr() + opt._at[i]
+                t.me, t.ve = opt._me.data_ptr() + opt._block[i], opt._ve.data_ptr() + opt._block[i]
+            t.ema = opt.ema.data_ptr() + 4 * opt._index[i] if opt.ema is not None else None
+        h = C.c_void_p()
+        L.check(L.lib().sr_adamw_create(L.dtype_code(self.dtype), self.bits, self.n, arr, C.byref(h)), 'sr_adamw_create')
+        tracked = _host_lib().srt_track(self.params)
+        if not tracked:
+            L.lib().sr_adamw_destroy(h)
+            _host_failed('AdamW')
+        old = (self.handle, self.tracked)
+        self.handle, self.tracked = h, tracked
+        if opt.capturable and old[0]:
+            self.retired.append(old)   # a captured graph may still read the tables
+        else:
+            self._free(*old)
+
+    @staticmethod
+    def _free(handle, tracked):
+        if handle:
+            L.lib().sr_adamw_destroy(handle)
+        if tracked:
+            _host_lib().srt_untrack(tracked)
+
+    def __del__(self):
+        try:
+            for pair in self.retired + [(self.handle, self.tracked)]:
+                self._free(*pair)
+        except Exception:   # interpreter shutdown
+            pass
+
+    def gradients(self, keep):
+        """Fills self.ptrs; returns the number of tensors without a gradient.  keep: copies that must live until the launch."""
+        missing = _host_lib().srt_gradients(self.tracked, self.ptrs, self.odd, C.byref(self.nodd), C.byref(self.moved))
+        if missing < 0:
+            _host_failed('AdamW')
+        for k in range(self.nodd.value):
+            p = self.params[self.odd[k]]
+            g = p.grad
+            if g.layout != torch.strided or g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
+                raise RuntimeError('AdamW: the gradient of parameter %d (%s %s on %s) does not fit it (%s %s on %s)'
+                                   % (self.members[self.odd[k]], tuple(g.shape), g.dtype, g.device, tuple(p.shape), p.dtype, p.device))
+            g = torch.empty_like(p).copy_(g)
+            keep.append(g)
+            self.ptrs[self.odd[k]] = g.data_ptr()
+        return missing
+
+    def table(self, dev, ptrs=None):
+        ptrs = self.ptrs if ptrs is None else ptrs
+        return _upload(8 * self.n, lambda at: C.memmove(at, ptrs, 8 * self.n), dev)
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW (decoupled weight decay, no amsgrad) as one hand-written kernel per parameter group, for groups of any
+    number of tensors; moments in float32 or, with `state_bits=8` (per group), in 8 bits each.
+
+        opt = AdamW(net.parameters(), lr=1e-4, state_bits=8, ema_decay=0.999)
+        ...
+        loss.backward()
+        opt.step(clip_grad_norm=1.0)          # or train.train_step(net, opt, ...)
+
+    Parameters: float32 or bfloat16, dense, on one GPU; they stay where they are.  bfloat16 parameters are rounded
+    stochastically (an update of 1e-4 of a weight is below half a bfloat16 step and would be lost).  8-bit moments: 256 values share an
+    exponent byte, m and v have three mantissa bits each and are rounded stochastically (rounded to nearest, v would not move under
+    beta2 = 0.999); 2.01 bytes of state a parameter instead of 8.  The random bits are a hash of (seed, step, element): two runs
+    give the same bits, whatever the launch.
+
+    ema_decay: keeps `opt.ema`, a float32 average of the weights (ema = d ema + (1 - d) p after every step, in the same
+    kernel); `ema_parameters()` gives it tensor by tensor, for a `params_ema` checkpoint.
+    clip_grad_norm in step(): the global norm of all gradients, its factor applied as the gradients are read (they are not
+    written back); `opt.grad_norm` holds the norm afterwards, on the device.  Nothing in step() waits for the GPU.
+    In a process group of more than one rank step() all-reduces the gradients first (train.allreduce_gradients), and the
+    constructor broadcasts rank 0's parameters (`broadcast=False`: not).
+
+    Parameters without a gradient are skipped, with their own step count, as torch does; their average goes on.
+    state_dict() / load_state_dict() use torch.optim.AdamW's layout (float32 `exp_avg`, `exp_avg_sq`, `step`; plus `ema`), so a
+    checkpoint moves between the two and between 32 and 8 bits; values that 8 bits hold come back as they were.
+    capturable=True: the step count (and an lr given as a float32 GPU tensor) live on the device, for steps inside a captured
+    graph; every step then has to bring the same gradients.  Without it a step under capture raises."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, ema_decay=None, seed=0, capturable=False,
+                 broadcast=True, group=None):
+        if ema_decay is not None and not 0.0 <= ema_decay <= 1.0:
+            raise ValueError('AdamW: ema_decay must lie in [0, 1] (got %r)' % (ema_decay,))
+        self._built = False
+        self.capturable, self.ema_decay, self.seed = bool(capturable), ema_decay, int(seed) & (1 << 64) - 1
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+        self.params = [p for g in self.param_groups for p in g['params']]
+        if not self.params:
+            raise ValueError('AdamW: no parameters')
+        self.device = dev = self.params[0].device
+        for g in self.param_groups:
+            self._hyper(g)
+        for p in self.params:
+            L.require_gpu(p, 'AdamW')
+            if p.dtype not in (torch.float32, torch.bfloat16) or p.device != dev:
+                raise TypeError('AdamW: float32 or bfloat16 parameters on one GPU')
+            if not _is_dense(p):
+                raise ValueError('AdamW: a parameter with holes or repeated elements')
+        self._check_overlap()
+        # places: element number among all parameters; offset among the tensors of the same kind of moments; first block
+        self._index, self._at, self._block, total, n = [], [], [], 0, {32: 0, 8: 0}
+        blocks = 0
+        for g in self.param_groups:
+            for p in g['params']:
+                k = p.numel()
+                self._index.append(total)
+                self._at.append(n[g['state_bits']])
+                self._block.append(blocks)
+                total += k
+                n[g['state_bits']] += k
+                blocks += -(-k // L.ADAMW_BLOCK) if g['state_bits'] == 8 else 0
+        self.numel = total
+        with torch.cuda.device(dev), torch.no_grad():
+            if broadcast and _world(group) > 1:
+                _broadcast_parameters(self.params, group)
+            self._m32, self._v32 = (torch.zeros(n[32], dtype=torch.float32, device=dev) for _ in range(2))
+            self._m8, self._v8 = (torch.zeros(n[8], dtype=torch.uint8, device=dev) for _ in range(2))
+            self._me, self._ve = (torch.ones(blocks, dtype=torch.uint8, device=dev) for _ in range(2))
+            self.ema = None
+            if ema_decay is not None:
+                self.ema = torch.empty(total, dtype=torch.float32, device=dev)
+                self._reset_ema()
+            self._lists, first = [], 0
+            for g in self.param_groups:
+                for dt in (torch.float32, torch.bfloat16):
+                    members = [first + i for i, p in enumerate(g['params']) if p.dtype == dt]
+                    if members:
+                        self._lists.append(_List(self, g, g['state_bits'], members))
+                first += len(g['params'])
+            if len(self._lists) > L.GRAD_MAX_LISTS:
+                raise ValueError('AdamW: at most %d parameter groups of one dtype' % L.GRAD_MAX_LISTS)
+            for lst in self._lists:
+                lst.build(self)
+        self.grad_norm = None   # of the last step with clip_grad_norm
+        self._built = True
+
+    def add_param_group(self, param_group):
+        if self._built:
+            raise RuntimeError('AdamW: give all parameter groups to the constructor (the moments of all tensors are laid out there)')
+        bits = param_group.get('state_bits', self.defaults['state_bits'])
+        if bits not in (32, 8):
+            raise ValueError('AdamW: state_bits is 32 or 8 (got %r)' % (bits,))
+        super().add_param_group(param_group)
+        ps = self.param_groups[-1]['params']
+        if len({id(p) for p in ps}) != len(ps):
+            raise ValueError('AdamW: a parameter appears twice')
+
+    def __getstate__(self):   # copy and pickle
+        raise TypeError('AdamW holds device tables and cannot be copied or pickled: keep its state_dict()')
+
+    # ---- state ---------------------------------------------------------------------------------------------------------
+    def _hyper(self, g):
+        lr, (b1, b2) = g['lr'], g['betas']
+        if torch.is_tensor(lr):
+            if lr.numel() != 1:
+                raise ValueError('AdamW: lr must have one element')
+            if self.capturable and lr.is_cuda:
+                if lr.dtype != torch.float32 or lr.device != self.device:
+                    raise TypeError("AdamW: a learning rate on the GPU is float32, on the parameters' device")
+                lr = 0.0   # the kernel reads it
+            else:
+                lr = float(lr)
+        if not (lr >= 0 and 0 <= b1 < 1 and 0 <= b2 < 1 and g['eps'] >= 0 and g['weight_decay'] >= 0):
+            raise ValueError('AdamW: lr %r, betas %r, eps %r, weight_decay %r out of range' % (g['lr'], g['betas'], g['eps'], g['weight_decay']))
+        return L.AdamWHyper(lr, b1, b2, g['eps'], g['weight_decay'], self.ema_decay or 0.0, self.seed)
+
+    def _reset_ema(self):
+        for p, at in zip(self.params, self._index):
+            self.ema[at:at + p.numel()].copy_(self._flat(p))
+
+    @staticmethod
+    def _flat(t):
+        """A dense tensor's elements in memory order."""
+        return t.detach().as_strided((t.numel(),), (1,))
+
+    def _shaped(self, flat, i):
+        """Tensor i's part of a flat array, in the parameter's shape and strides."""
+        p = self.params[i]
+        return flat[self._index[i]:self._index[i] + p.numel()].as_strided(p.shape, p.stride())
+
+    @property
+    def exp_avg(self):
+        """The first moments of all parameters as one flat float32 buffer, in the order of the parameters (32-bit moments)."""
+        if self._m8.numel():
+            raise RuntimeError('AdamW: with 8-bit moments use moments()')
+        return self._m32
+
+    @property
+    def exp_avg_sq(self):
+        if self._v8.numel():
+            raise RuntimeError('AdamW: with 8-bit moments use moments()')
+        return self._v32
+
+    def moments(self, dtype=torch.float32):
+        """(exp_avg, exp_avg_sq) of all parameters as new flat tensors, in the order of the parameters; 8-bit moments as the values
+        that their codes stand for (bfloat16 holds those of m and v exactly, within its range)."""
+        code = L.dtype_code(dtype)
+        with torch.cuda.device(self.device):
+            m, v = (torch.empty(self.numel, dtype=dtype, device=self.device) for _ in range(2))
+            for lst in self._lists:
+                if self.numel:
+                    L.check(L.lib().sr_adamw_moments(lst.handle, code, m.data_ptr(), v.data_ptr(), L.stream_ptr(self.device)), 'sr_adamw_moments')
+        return m, v
+
+    def ema_parameters(self):
+        """The average of the weights, one float32 view of `ema` per parameter."""
+        if self.ema is None:
+            raise RuntimeError('AdamW: built without ema_decay')
+        return [self._shaped(self.ema, i) for i in range(len(self.params))]
+
+    # ---- step ----------------------------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None, group=None, average=True, clip_grad_norm=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if _world(group) > 1:
+            _exchange_gradients(self.params, group, average)
+        if clip_grad_norm is not None and not clip_grad_norm >= 0:
+            raise ValueError('AdamW: clip_grad_norm must not be negative (got %r)' % (clip_grad_norm,))
+        dev = self.device
+        with torch.cuda.device(dev):
+            capturing = torch.cuda.is_current_stream_capturing()
+            if capturing and not self.capturable:
+                raise RuntimeError('AdamW: a step under graph capture needs capturable=True (the step count would stay what it is now)')
+            keep, hypers, missing = [], [], []
+            for lst in self._lists:   # everything that can fail comes before the first launch
+                hypers.append(self._hyper(lst.group))
+                missing.append(lst.gradients(keep))
+                if lst.moved.value:
+                    self._follow(lst, capturing)
+                if self.capturable and missing[-1] < lst.n:
+                    self._same_gradients(lst)
+            tables = [lst.table(dev) for lst in self._lists]
+            factor = None
+            if clip_grad_norm is not None:
+                lists = (L.GradList * len(self._lists))()
+                for l, lst, table in zip(lists, self._lists, tables):
+                    l.list, l.grads = lst.handle, table.data_ptr()
+                out = _norm(lists, float(clip_grad_norm), dev)
+                self.grad_norm, factor = out[0], out.data_ptr() + 4
+            for lst, h, miss, table in zip(self._lists, hypers, missing, tables):
+                self._launch(lst, h, miss, table, factor)
+                if _host_lib().srt_written(lst.tracked, lst.ptrs if miss else None) < 0:
+                    _host_failed('AdamW')
+        return loss
+
+    def _launch(self, lst, h, missing, table, factor):
+        lib, st = L.lib(), L.stream_ptr(self.device)
+
+        def run(step, scalars, grads):
+            L.check(lib.sr_adamw_step(lst.handle, C.byref(h), step, scalars, grads.data_ptr(), factor, st), 'sr_adamw_step')
+        if missing == lst.n:
+            if self.ema is not None:
+                run(1, None, table)
+            return
+        if self.capturable:
+            lr = lst.group['lr']
+            L.check(lib.sr_adamw_tick(C.byref(h), lr.data_ptr() if torch.is_tensor(lr) and lr.is_cuda else None, lst.step_dev.data_ptr(),
+                                      lst.scalars.data_ptr(), st), 'sr_adamw_tick')
+            run(0, lst.scalars.data_ptr(), table)
+            return
+        if not missing and isinstance(lst.steps, int):
+            lst.steps += 1
+            run(lst.steps, None, table)
+            return
+        # step counts differ: one launch per count, the other tensors marked; the first one also takes those without a gradient
+        # (their averages)
+        ptrs = np.frombuffer(lst.ptrs, dtype=np.uint64)
+        have = ptrs != 0
+        steps = np.full(lst.n, lst.steps, dtype=np.int64) if isinstance(lst.steps, int) else lst.steps
+        lst.steps = steps = steps + have
+        rest = ~have
+        for t in np.unique(steps[have]):
+            now = have & (steps == t) | rest
+            rest = np.zeros_like(rest)
+            part = np.where(now, ptrs, np.uint64(L.ADAMW_SKIP))
+            run(int(t), None, lst.table(self.device, part.ctypes.data))
+        if (steps == steps[0]).all():
+            lst.steps = int(steps[0])
+
+    def _follow(self, lst, capturing):
+        """Parameters lie elsewhere (`.data =`): same dtype, device and size are followed, anything else is refused."""
+        for p, n in zip(lst.params, lst.sizes):
+            if p.device != self.device or p.dtype != lst.dtype or p.numel() != n or not _is_dense(p):
+                raise RuntimeError('AdamW: a parameter was moved, cast or resized after the optimizer was built -- rebuild the optimizer')
+        if capturing:
+            raise RuntimeError('AdamW: a parameter was re-pointed; run one step outside the capture first')
+        self._check_overlap()
+        lst.build(self)
+
+    def _check_overlap(self):
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+            raise ValueError('AdamW: two parameters share memory')
+
+    def _same_gradients(self, lst):
+        """One step count on the device serves all tensors of a list."""
+        have = np.frombuffer(lst.ptrs, dtype=np.uint64) != 0
+        if lst.seen is None:
+            lst.seen = have
+        elif not np.array_equal(lst.seen, have):
+            raise RuntimeError('AdamW(capturable=True): a step must bring gradients for the same parameters as the one before')
+
+    # ---- checkpoints ---------------------------------------------------------------------------------------------------
+    def _steps_of(self, lst):
+        if self.capturable:
+            t = int(lst.step_dev.item())
+            return [t if lst.seen is None or lst.seen[i] else 0 for i in range(lst.n)]
+        return [lst.steps] * lst.n if isinstance(lst.steps, int) else lst.steps.tolist()
+
+    def state_dict(self):
+        """torch.optim.AdamW's layout: {'state': {i: {'step', 'exp_avg', 'exp_avg_sq'[, 'ema']}}, 'param_groups': [...]}."""
+        steps = {}
+        for lst in self._lists:
+            steps.update(zip(lst.members, self._steps_of(lst)))
+        state = {}
+        if any(steps.values()):
+            m, v = self.moments()
+            ema = self.ema.clone() if self.ema is not None else None
+            for i in range(len(self.params)):
+                if steps[i]:
+                    state[i] = {'step': torch.tensor(float(steps[i])), 'exp_avg': self._shaped(m, i), 'exp_avg_sq': self._shaped(v, i)}
+                if ema is not None:
+                    state.setdefault(i, {})['ema'] = self._shaped(ema, i)
+        groups, first = [], 0
+        for g in self.param_groups:
+            hp = {k: x for k, x in g.items() if k != 'params'}
+            hp['params'] = list(range(first, first + len(g['params'])))
+            first += len(g['params'])
+            groups.append(hp)
+        return {'state': state, 'param_groups': groups}
+
+    @torch.no_grad()
+    def load_state_dict(self, sd):
+        groups = sd['param_groups']
+        if [len(g['params']) for g in groups] != [len(g['params']) for g in self.param_groups]:
+            raise ValueError('AdamW.load_state_dict: expected groups of %s parameters' % [len(g['params']) for g in self.param_groups])
+        for g in groups:
+            if g.get('amsgrad') or g.get('maximize'):
+                raise ValueError('AdamW.load_state_dict: amsgrad and maximize are not supported')
+        place = {}
+        for i, key in enumerate(k for g in groups for k in g['params']):
+            place[key] = i
+        state = {place[k]: s for k, s in sd['state'].items()}
+        for i, s in state.items():
+            for name in ('exp_avg', 'exp_avg_sq', 'ema'):
+                if name in s and tuple(s[name].shape) != tuple(self.params[i].shape):
+                    raise ValueError('AdamW.load_state_dict: parameter %d has shape %s, its %s %s'
+                                     % (i, tuple(self.params[i].shape), name, tuple(s[name].shape)))
+        new = [{k: g.get(k, mine[k]) for k in ('lr', 'betas', 'eps', 'weight_decay')} for g, mine in zip(groups, self.param_groups)]
+        for hp in new:
+            self._hyper(hp)
+        for mine, hp in zip(self.param_groups, new):
+            mine.update(hp)
+
+        def flat(name, i):
+            p, x = self.params[i], state.get(i, {}).get(name)
+            if x is None:
+                return torch.zeros(p.numel(), dtype=torch.float32, device=self.device)
+            x = x.detach().to(self.device, torch.float32)
+            return self._flat(x if x.stride() == p.stride() else torch.empty_like(p, dtype=torch.float32).copy_(x))
+        with torch.cuda.device(self.device):
+            if self.numel:
+                m, v = (torch.cat([flat(name, i) for i in range(len(self.params))]) for name in ('exp_avg', 'exp_avg_sq'))
+                for lst in self._lists:
+                    L.check(L.lib().sr_adamw_set_moments(lst.handle, m.data_ptr(), v.data_ptr(), self.seed, L.stream_ptr(self.device)),
+                            'sr_adamw_set_moments')
+            for lst in self._lists:
+                steps = np.array([int(float(state.get(i, {}).get('step', 0))) for i in lst.members], dtype=np.int64)
+                if self.capturable:
+                    t = int(steps.max())
+                    if not all(k in (0, t) for k in steps.tolist()):
+                        raise ValueError('AdamW.load_state_dict: capturable=True takes one step count')
+                    lst.step_dev.fill_(t)
+                    lst.seen = None
+                else:
+                    lst.steps = int(steps[0]) if (steps == steps[0]).all() else steps
+            if self.ema is not None:
+                self._reset_ema()
+                for i, s in state.items():
+                    if 'ema' in s:
+                        self.ema[self._index[i]:self._index[i] + self.params[i].numel()].copy_(flat('ema', i))

@@ -32,6 +32,7 @@ import torch.nn.functional as F
 
 from . import _lib as L
 from .fdconv import FDConv
+from .optim import AdamW, clip_grad_norm_  # noqa: F401
 
 BN_EPS = 1e-5
 
@@ -976,7 +977,7 @@ def train_step(net, optimizer, wf, sr, weighted=False, sigmoid=False, clip_grad_
         loss = loss + perceptual_loss(pred, sr, perceptual['vgg'], perceptual.get('layer_weights'), perceptual.get('weight', 1.0),
                                       perceptual.get('compute_dtype', torch.bfloat16))
     loss.backward()
-    if isinstance(optimizer, FlatAdam):  # gathers, all-reduces and clips the flat gradient itself
+    if isinstance(optimizer, (FlatAdam, AdamW)):  # all-reduces and clips by itself
         optimizer.step(group=group, clip_grad_norm=clip_grad_norm)
         return loss.detach()
     allreduce_gradients(net.parameters(), group=group)
