@@ -90,6 +90,13 @@ __device__ __forceinline__ uint32_t mix(uint32_t lo, uint32_t hi_c, uint32_t k0,
     return x ^ (x >> 16);
 }
 
+// pointers that come out of a table are of no known address space, and FLAT instructions (which also wait for LDS) would follow
+#define GLOBAL __attribute__((address_space(1)))
+template <typename T>
+__device__ __forceinline__ GLOBAL T* global(const void* p) {
+    return (GLOBAL T*)const_cast<void*>(p);
+}
+
 // vectors with the alignment of their elements: tensors are views at any offset (the gradients of one layer are pieces of one
 // buffer); the hardware loads and stores 16 bytes at any address
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -97,53 +104,53 @@ typedef uint16_t h4u __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint8_t b4u __attribute__((ext_vector_type(4), aligned(1)));
 
 // 4 values at p, of which the first cnt exist (the others: 0)
-__device__ __forceinline__ void load4(const float* p, int cnt, float (&r)[4]) {
+__device__ __forceinline__ void load4(const GLOBAL float* p, int cnt, float (&r)[4]) {
     if (cnt >= 4) {
-        const f4u x = *(const f4u*)p;
+        const f4u x = *(const GLOBAL f4u*)p;
         r[0] = x.x, r[1] = x.y, r[2] = x.z, r[3] = x.w;
     } else {
         r[0] = cnt > 0 ? p[0] : 0.f, r[1] = cnt > 1 ? p[1] : 0.f, r[2] = cnt > 2 ? p[2] : 0.f, r[3] = 0.f;
     }
 }
-__device__ __forceinline__ void load4(const bf16_t* p, int cnt, float (&r)[4]) {
+__device__ __forceinline__ void load4(const GLOBAL bf16_t* p, int cnt, float (&r)[4]) {
     if (cnt >= 4) {
-        const h4u x = *(const h4u*)p;
+        const h4u x = *(const GLOBAL h4u*)p;
         r[0] = bf16_to_f32(x.x), r[1] = bf16_to_f32(x.y), r[2] = bf16_to_f32(x.z), r[3] = bf16_to_f32(x.w);
     } else {
         r[0] = cnt > 0 ? bf16_to_f32(p[0]) : 0.f, r[1] = cnt > 1 ? bf16_to_f32(p[1]) : 0.f, r[2] = cnt > 2 ? bf16_to_f32(p[2]) : 0.f, r[3] = 0.f;
     }
 }
-__device__ __forceinline__ void store4(float* p, int cnt, const float (&r)[4]) {
+__device__ __forceinline__ void store4(GLOBAL float* p, int cnt, const float (&r)[4]) {
     if (cnt >= 4) {
         const f4u x = {r[0], r[1], r[2], r[3]};
-        *(f4u*)p = x;
+        *(GLOBAL f4u*)p = x;
     } else {
         if (cnt > 0) p[0] = r[0];
         if (cnt > 1) p[1] = r[1];
         if (cnt > 2) p[2] = r[2];
     }
 }
-__device__ __forceinline__ void store4(bf16_t* p, int cnt, const uint16_t (&r)[4]) {
+__device__ __forceinline__ void store4(GLOBAL bf16_t* p, int cnt, const uint16_t (&r)[4]) {
     if (cnt >= 4) {
         const h4u x = {r[0], r[1], r[2], r[3]};
-        *(h4u*)p = x;
+        *(GLOBAL h4u*)p = x;
     } else {
         if (cnt > 0) p[0] = r[0];
         if (cnt > 1) p[1] = r[1];
         if (cnt > 2) p[2] = r[2];
     }
 }
-__device__ __forceinline__ uint32_t load4b(const uint8_t* p, int cnt) {  // byte j of the result: code j
-    if (cnt >= 4) return __builtin_bit_cast(uint32_t, *(const b4u*)p);
+__device__ __forceinline__ uint32_t load4b(const GLOBAL uint8_t* p, int cnt) {  // byte j of the result: code j
+    if (cnt >= 4) return __builtin_bit_cast(uint32_t, *(const GLOBAL b4u*)p);
     uint32_t r = 0;
     if (cnt > 0) r = p[0];
     if (cnt > 1) r |= (uint32_t)p[1] << 8;
     if (cnt > 2) r |= (uint32_t)p[2] << 16;
     return r;
 }
-__device__ __forceinline__ void store4b(uint8_t* p, int cnt, uint32_t x) {
+__device__ __forceinline__ void store4b(GLOBAL uint8_t* p, int cnt, uint32_t x) {
     if (cnt >= 4) {
-        *(b4u*)p = __builtin_bit_cast(b4u, x);
+        *(GLOBAL b4u*)p = __builtin_bit_cast(b4u, x);
     } else {
         if (cnt > 0) p[0] = (uint8_t)x;
         if (cnt > 1) p[1] = (uint8_t)(x >> 8);
@@ -174,76 +181,129 @@ __device__ __forceinline__ uint32_t block_exponent(uint32_t top) {
 }
 constexpr int M_BIAS = 112, V_BIAS = 96;  // where the exponent field of the block's largest value lies: 127 - 15, 127 - 31
 
-__device__ __forceinline__ float decode_m(uint32_t code, uint32_t eb) {
-    const float x = ldexpf(__uint_as_float((code & 0x7F) << 20), (int)eb - 127 + M_BIAS);
-    const float y = eb == 255 ? __uint_as_float(0x7FC00000u) : x;
-    return __uint_as_float(__float_as_uint(y) | (code & 0x80) << 24);
+// the four codes in a word -> values
+__device__ __forceinline__ void decode4_m(uint32_t c, uint32_t eb, float (&m)[4]) {
+    const int e = (int)eb - 127 + M_BIAS;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int t = (int)(c << (24 - 8 * j)) >> 4;  // sign in 27 .. 31, the other bits in 20 .. 26, other codes below
+        m[j] = ldexpf(__uint_as_float((uint32_t)t & 0x87F00000u), e);
+    }
+    if (eb == 255) m[0] = m[1] = m[2] = m[3] = __uint_as_float(0x7FC00000u);
 }
-__device__ __forceinline__ float decode_v(uint32_t code, uint32_t eb) {
-    const float x = ldexpf(__uint_as_float(code << 20), (int)eb - 127 + V_BIAS);
-    return eb == 255 ? __uint_as_float(0x7FC00000u) : x;
+__device__ __forceinline__ void decode4_v(uint32_t c, uint32_t eb, float (&v)[4]) {
+    const int e = (int)eb - 127 + V_BIAS;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = ldexpf(__uint_as_float((c >> 8 * j & 0xFF) << 20), e);
+    if (eb == 255) v[0] = v[1] = v[2] = v[3] = __uint_as_float(0x7FC00000u);
 }
-// noise: 16 random bits; they take the upper 16 of the 20 that are cut, the middle of what is below stands for the rest
-__device__ __forceinline__ uint32_t encode_m(float m, uint32_t eb, uint32_t noise) {
-    const uint32_t u = __float_as_uint(m);
-    const uint32_t y = __float_as_uint(ldexpf(__uint_as_float(u & 0x7FFFFFFFu), 127 - M_BIAS - (int)eb));
-    return eb == 255 ? 0 : ((y + (noise << 4 | 8)) >> 20) | (u >> 31) << 7;
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t (&w)[4]) {
+    return __builtin_amdgcn_perm(w[1], w[0], 0x0C0C0703u) | __builtin_amdgcn_perm(w[3], w[2], 0x07030C0Cu);
 }
-__device__ __forceinline__ uint32_t encode_v(float v, uint32_t eb, uint32_t noise) {
-    const uint32_t y = __float_as_uint(ldexpf(fabsf(v), 127 - V_BIAS - (int)eb));
-    const uint32_t c = (y + (noise << 4 | 8)) >> 20;
-    return eb == 255 ? 0 : c == 0 && v > 0.f ? 1 : c;
-}
-// the four values of every lane of one block -> codes (byte j: value j) and the block's exponent byte; lanes past the end hold 0
-__device__ __forceinline__ uint32_t encode4_m(const float (&m)[4], const uint32_t (&h)[4], uint32_t& eb) {
+// the largest magnitude of a wave's 4 * 64 values, as bits
+__device__ __forceinline__ uint32_t block_top(const float (&x)[4]) {
     uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(m[j]) & 0x7FFFFFFFu);
-    eb = block_exponent(wave_max(top));
-    uint32_t c = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c |= encode_m(m[j], eb, h[j] & 0xFFFF) << 8 * j;
-    return c;
+    for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[j]) << 1);
+    return wave_max(top) >> 1;
 }
-__device__ __forceinline__ uint32_t encode4_v(const float (&v)[4], const uint32_t (&h)[4], uint32_t& eb) {
-    uint32_t top = 0;
+// Values -> codes (byte j: value j).  The float of a code's place in the format, shifted left by four, has the code in its top
+// byte; below it come 16 random bits and the middle of what is finer.  Nothing carries out: block_exponent left room.
+__device__ __forceinline__ uint32_t encode4_m(const float (&m)[4], uint32_t eb, const uint32_t (&h)[4]) {
+    const int e = 127 - M_BIAS - (int)eb;
+    uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-    eb = block_exponent(wave_max(top));
-    uint32_t c = 0;
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t y = (__float_as_uint(ldexpf(fabsf(m[j]), e)) << 4) + __builtin_amdgcn_perm(h[j], 0x80u, 0x0C050400u);
+        w[j] = (y & 0x7FFFFFFFu) | (__float_as_uint(m[j]) & 0x80000000u);
+    }
+    return eb == 255 ? 0 : top_bytes(w);
+}
+__device__ __forceinline__ uint32_t encode4_v(const float (&v)[4], uint32_t eb, const uint32_t (&h)[4]) {
+    const int e = 127 - V_BIAS - (int)eb;
+    uint32_t w[4], least = ~0u;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) c |= encode_v(v[j], eb, h[j] >> 16) << 8 * j;
-    return c;
+    for (int j = 0; j < 4; ++j) {
+        w[j] = (__float_as_uint(ldexpf(fabsf(v[j]), e)) << 4) + __builtin_amdgcn_perm(h[j], 0x80u, 0x0C070600u);
+        least = min(least, w[j]);
+    }
+    if (least < 1u << 24) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (w[j] < 1u << 24 && v[j] > 0.f) w[j] = 1u << 24;
+    }
+    return eb == 255 ? 0 : top_bytes(w);
 }
 __device__ __forceinline__ void hash4(uint64_t at, const Scalars& s, uint32_t (&h)[4]) {
+    const uint32_t lo = (uint32_t)at, c = (uint32_t)(at >> 32) * GOLDEN;
+    if (lo < 0xFFFFFFFCu) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = mix((uint32_t)(at + j), (uint32_t)((at + j) >> 32) * GOLDEN, s.k0, s.k1);
+        for (int j = 0; j < 4; ++j) h[j] = mix(lo + j, c, s.k0, s.k1);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = mix((uint32_t)(at + j), (uint32_t)((at + j) >> 32) * GOLDEN, s.k0, s.k1);
+    }
 }
-// stochastic rounding to bfloat16; infinities and NaN as they are
+// stochastic rounding to bfloat16; infinities and (quiet) NaN as they are
 __device__ __forceinline__ uint16_t round_bf16(float x, uint32_t h) {
-    const uint32_t u = __float_as_uint(x);
-    const bool finite = (u & 0x7F800000u) != 0x7F800000u;
-    const uint32_t r = finite ? u + ((h * GOLDEN) >> 16) : u | ((u & 0xFFFF) ? 0x400000u : 0);
-    return (uint16_t)(r >> 16);
+    const uint32_t noise = __builtin_isfinite(x) ? (h * GOLDEN) >> 16 : 0;
+    return (uint16_t)((__float_as_uint(x) + noise) >> 16);
 }
 
-__device__ __forceinline__ void update4(const Scalars& s, float factor, float (&p)[4], const float (&g)[4], float (&m)[4], float (&v)[4]) {
+// Square root and quotient, correctly rounded as sqrtf and `/` are, without their handling of the ends of the range: half the
+// instructions, which is what bounds the step with 8-bit moments.  rsq / rcp are good to one ulp; one correction by the exact
+// residual rounds the root correctly (checked for all 2^24 significands) and the reciprocal (all 2^23), and with a correctly
+// rounded reciprocal the same correction rounds the quotient correctly (Markstein's theorem).  The ranges below keep every
+// residual exact: 0 <= x < 2^124, no subnormals but 0; |a| 0 or in [2^-85, 2^84], b in [2^-40, 2^31].
+__device__ __forceinline__ float root(float x) {
+    const float y = __builtin_amdgcn_rsqf(fmaxf(x, 0x1p-100f));
+    const float r = x * y;
+    return fmaf(fmaf(-r, r, x), 0.5f * y, r);
+}
+__device__ __forceinline__ float quotient(float a, float b) {
+    float r = __builtin_amdgcn_rcpf(b);
+    r = fmaf(fmaf(-b, r, 1.f), r, r);
+    const float q = a * r;
+    return fmaf(fmaf(-b, q, a), r, q);
+}
+
+__device__ __forceinline__ void moments4(const Scalars& s, float factor, const float (&g)[4], float (&m)[4], float (&v)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const float gj = g[j] * factor;
         m[j] = m[j] * s.b1 + gj * s.c1;
         v[j] = v[j] * s.b2 + (gj * gj) * s.c2;
-        p[j] = p[j] * s.decay - (m[j] / (sqrtf(v[j]) * s.rbc2 + s.eps)) * s.step_size;
     }
+}
+__device__ __forceinline__ void weights4(const Scalars& s, float (&p)[4], const float (&m)[4], const float (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = p[j] * s.decay - (m[j] / (sqrtf(v[j]) * s.rbc2 + s.eps)) * s.step_size;
+}
+// The same for v < 2^60, |m| < 2^20 and eps >= 2^-40, as a block's exponents tell.  v and m are raised by 2^64 first (which keeps
+// subnormals in range) and the constants that follow take it back: exact, so the results are the same bits unless the quotient
+// itself is subnormal, where this one does not round it and the update is below 2^-126.
+__device__ __forceinline__ void weights4_in_range(const Scalars& s, float (&p)[4], const float (&m)[4], const float (&v)[4]) {
+    const float rbc2 = s.rbc2 * 0x1p-32f, step_size = s.step_size * 0x1p-64f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = p[j] * s.decay - quotient(m[j] * 0x1p64f, root(v[j] * 0x1p64f) * rbc2 + s.eps) * step_size;
 }
 
 template <typename P, int BITS, bool FULL>
-__device__ __forceinline__ void step_piece(const Rec& r, const P* gp, const Scalars& s, float factor, int64_t off, int left, int lane) {
+__device__ __forceinline__ void step_piece(const Rec& r, const void* grad, const Scalars& s, float factor, int64_t off, int left, int lane) {
     constexpr int GROUPS = PIECE / 256;
-    P* pp = (P*)r.p + off;
-    gp += off;
+    GLOBAL P* pp = global<P>(r.p) + off;
+    const GLOBAL P* gp = global<P>(grad) + off;
+    GLOBAL float* ep = global<float>(r.ema) + off;
+    GLOBAL float *m32 = global<float>(r.m) + off, *v32 = global<float>(r.v) + off;
+    GLOBAL uint8_t *m8 = global<uint8_t>(r.m) + off, *v8 = global<uint8_t>(r.v) + off;
+    GLOBAL uint8_t *me = global<uint8_t>(r.me) + off / QBLOCK, *ve = global<uint8_t>(r.ve) + off / QBLOCK;
     float p[GROUPS][4], g[GROUPS][4], m[GROUPS][4], v[GROUPS][4], e[GROUPS][4];
     uint32_t mc[GROUPS], vc[GROUPS], meb[GROUPS], veb[GROUPS];
+    if (BITS == 8 && FULL) {  // four exponents at once
+        const uint32_t a = __builtin_amdgcn_readfirstlane(load4b(me, 4)), b = __builtin_amdgcn_readfirstlane(load4b(ve, 4));
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) meb[k] = a >> 8 * k & 0xFF, veb[k] = b >> 8 * k & 0xFF;
+    }
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k) {
         if (!FULL && k * 256 >= left) break;
@@ -251,32 +311,47 @@ __device__ __forceinline__ void step_piece(const Rec& r, const P* gp, const Scal
         load4(pp + at, cnt, p[k]);
         load4(gp + at, cnt, g[k]);
         if (BITS == 32) {
-            load4((const float*)r.m + off + at, cnt, m[k]);
-            load4((const float*)r.v + off + at, cnt, v[k]);
+            load4(m32 + at, cnt, m[k]);
+            load4(v32 + at, cnt, v[k]);
         } else {
-            mc[k] = load4b((const uint8_t*)r.m + off + at, cnt);
-            vc[k] = load4b((const uint8_t*)r.v + off + at, cnt);
-            meb[k] = r.me[off / QBLOCK + k];
-            veb[k] = r.ve[off / QBLOCK + k];
+            mc[k] = load4b(m8 + at, cnt);
+            vc[k] = load4b(v8 + at, cnt);
+            if (!FULL) meb[k] = __builtin_amdgcn_readfirstlane(me[k]), veb[k] = __builtin_amdgcn_readfirstlane(ve[k]);
         }
-        if (r.ema) load4(r.ema + off + at, cnt, e[k]);
+        if (r.ema) load4(ep + at, cnt, e[k]);
     }
+    uint32_t em = 0, ev = 0;  // the new exponents
 #pragma unroll
     for (int k = 0; k < GROUPS; ++k) {
         if (!FULL && k * 256 >= left) break;
         const int at = k * 256 + lane * 4, cnt = FULL ? 4 : left - at;
         if (BITS == 8) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                m[k][j] = decode_m(mc[k] >> 8 * j & 0xFF, meb[k]);
-                v[k][j] = decode_v(vc[k] >> 8 * j & 0xFF, veb[k]);
-            }
+            decode4_m(mc[k], meb[k], m[k]);
+            decode4_v(vc[k], veb[k], v[k]);
         }
-        update4(s, factor, p[k], g[k], m[k], v[k]);
+        moments4(s, factor, g[k], m[k], v[k]);
+        uint32_t a = 0, b = 0;
+        if (BITS == 8) {
+            if (!FULL) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {  // a lane past the end must not take part in the block's maximum
+                    m[k][j] = j < cnt ? m[k][j] : 0.f;
+                    v[k][j] = j < cnt ? v[k][j] : 0.f;
+                }
+            }
+            a = block_exponent(block_top(m[k]));
+            b = block_exponent(block_top(v[k]));
+            em |= a << 8 * k;
+            ev |= b << 8 * k;
+        }
+        if (BITS == 8 && a < 127 + 20 && b < 127 + 60 && s.eps >= 0x1p-40f)
+            weights4_in_range(s, p[k], m[k], v[k]);
+        else
+            weights4(s, p[k], m[k], v[k]);
         if (r.ema) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) e[k][j] = e[k][j] * s.d + p[k][j] * s.cd;
-            store4(r.ema + off + at, cnt, e[k]);
+            store4(ep + at, cnt, e[k]);
         }
         uint32_t h[4];
         if (BITS == 8 || sizeof(P) == 2) hash4((uint64_t)(r.index + off + at), s, h);
@@ -289,24 +364,17 @@ __device__ __forceinline__ void step_piece(const Rec& r, const P* gp, const Scal
             store4(pp + at, cnt, p[k]);
         }
         if (BITS == 32) {
-            store4((float*)r.m + off + at, cnt, m[k]);
-            store4((float*)r.v + off + at, cnt, v[k]);
+            store4(m32 + at, cnt, m[k]);
+            store4(v32 + at, cnt, v[k]);
         } else {
-            if (!FULL) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {  // a lane past the end must not take part in the block's maximum
-                    m[k][j] = j < cnt ? m[k][j] : 0.f;
-                    v[k][j] = j < cnt ? v[k][j] : 0.f;
-                }
-            }
-            uint32_t eb;
-            const uint32_t a = encode4_m(m[k], h, eb);
-            if (lane == 0) r.me[off / QBLOCK + k] = (uint8_t)eb;
-            const uint32_t b = encode4_v(v[k], h, eb);
-            if (lane == 0) r.ve[off / QBLOCK + k] = (uint8_t)eb;
-            store4b((uint8_t*)r.m + off + at, cnt, a);
-            store4b((uint8_t*)r.v + off + at, cnt, b);
+            store4b(m8 + at, cnt, encode4_m(m[k], a, h));
+            store4b(v8 + at, cnt, encode4_v(v[k], b, h));
         }
+    }
+    if (BITS == 8 && lane == 0) {
+        const int blocks = FULL ? GROUPS : (left + QBLOCK - 1) / QBLOCK;
+        store4b(me, blocks, em);
+        store4b(ve, blocks, ev);
     }
 }
 
@@ -326,18 +394,29 @@ __global__ __launch_bounds__(256) void adamw_step_kernel(const Rec* __restrict__
     if (gp == (const void*)SR_ADAMW_SKIP) return;
     const Rec r = recs[c.tensor];
     if (!gp && !r.ema) return;
-    const Scalars s = scalars_at ? *scalars_at : scalars;
-    const float factor = factor_at ? *factor_at : 1.f;
+    Scalars s = scalars;
+    if (scalars_at) s = *scalars_at;
+    float factor = 1.f;
+    if (factor_at) factor = *factor_at;
     const int64_t off = (int64_t)c.number * PIECE;
     const int left = r.n - off < PIECE ? (int)(r.n - off) : PIECE;
     if (!gp) {  // no gradient: the weights stay, their average goes on
-        for (int at = lane; at < left; at += 64) r.ema[off + at] = r.ema[off + at] * s.d + Elem<P>::ld((const P*)r.p + off + at) * s.cd;
+        GLOBAL float* e = global<float>(r.ema) + off;
+        const GLOBAL P* p = global<P>(r.p) + off;
+        for (int at = lane; at < left; at += 64) {
+            float w;
+            if constexpr (sizeof(P) == 2)
+                w = bf16_to_f32(p[at]);
+            else
+                w = p[at];
+            e[at] = e[at] * s.d + w * s.cd;
+        }
         return;
     }
     if (left == PIECE)
-        step_piece<P, BITS, true>(r, (const P*)gp, s, factor, off, left, lane);
+        step_piece<P, BITS, true>(r, gp, s, factor, off, left, lane);
     else
-        step_piece<P, BITS, false>(r, (const P*)gp, s, factor, off, left, lane);
+        step_piece<P, BITS, false>(r, gp, s, factor, off, left, lane);
 }
 
 // step counter and scalars of a captured step: the host's values are fixed at capture, these move with every replay
@@ -347,7 +426,50 @@ __global__ void adamw_tick_kernel(sr_adamw_hyper h, const float* lr, int64_t* st
     *out = make_scalars(h, lr ? (double)*lr : h.lr, t);
 }
 
-// moments as the values they stand for, at the tensors' places in one flat pair of arrays
+// Moments as the values they stand for, at the tensors' places in one flat pair of arrays.  Four values a lane and group, all
+// groups' loads first.
+template <typename TO>
+__device__ __forceinline__ void put4(GLOBAL TO* to, int cnt, const float (&x)[4]) {
+    if constexpr (sizeof(TO) == 2) {
+        uint16_t y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = f32_to_bf16(x[j]);
+        store4(to, cnt, y);
+    } else {
+        store4(to, cnt, x);
+    }
+}
+template <typename TO, int BITS, bool FULL>
+__device__ __forceinline__ void moments_piece(const Rec& r, int64_t off, int left, int lane, TO* mo, TO* vo) {
+    constexpr int GROUPS = PIECE / 256;
+    float m[GROUPS][4], v[GROUPS][4];
+    uint32_t mc[GROUPS], vc[GROUPS], a[GROUPS], b[GROUPS];
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+        if (!FULL && k * 256 >= left) break;
+        const int at = k * 256 + lane * 4, cnt = FULL ? 4 : left - at;
+        if (BITS == 32) {
+            load4(global<float>(r.m) + off + at, cnt, m[k]);
+            load4(global<float>(r.v) + off + at, cnt, v[k]);
+        } else {
+            mc[k] = load4b(global<uint8_t>(r.m) + off + at, cnt);
+            vc[k] = load4b(global<uint8_t>(r.v) + off + at, cnt);
+            a[k] = global<uint8_t>(r.me)[off / QBLOCK + k];
+            b[k] = global<uint8_t>(r.ve)[off / QBLOCK + k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+        if (!FULL && k * 256 >= left) break;
+        const int at = k * 256 + lane * 4, cnt = FULL ? 4 : left - at;
+        if (BITS == 8) {
+            decode4_m(mc[k], __builtin_amdgcn_readfirstlane(a[k]), m[k]);
+            decode4_v(vc[k], __builtin_amdgcn_readfirstlane(b[k]), v[k]);
+        }
+        put4(global<TO>(mo) + r.index + off + at, cnt, m[k]);
+        put4(global<TO>(vo) + r.index + off + at, cnt, v[k]);
+    }
+}
 template <typename TO, int BITS>
 __global__ __launch_bounds__(256) void adamw_moments_kernel(const Rec* __restrict__ recs, const Piece* __restrict__ pieces, uint32_t npieces,
                                                             TO* __restrict__ mo, TO* __restrict__ vo) {
@@ -358,34 +480,10 @@ __global__ __launch_bounds__(256) void adamw_moments_kernel(const Rec* __restric
     const Rec r = recs[c.tensor];
     const int64_t off = (int64_t)c.number * PIECE;
     const int left = r.n - off < PIECE ? (int)(r.n - off) : PIECE;
-#pragma unroll
-    for (int k = 0; k < PIECE / 256; ++k) {
-        const int at = k * 256 + lane * 4, cnt = left - at;
-        if (cnt <= 0) return;
-        float m[4], v[4];
-        if (BITS == 32) {
-            load4((const float*)r.m + off + at, cnt, m);
-            load4((const float*)r.v + off + at, cnt, v);
-        } else {
-            const uint32_t a = load4b((const uint8_t*)r.m + off + at, cnt), b = load4b((const uint8_t*)r.v + off + at, cnt);
-            const uint32_t ea = r.me[off / QBLOCK + k], eb = r.ve[off / QBLOCK + k];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                m[j] = decode_m(a >> 8 * j & 0xFF, ea);
-                v[j] = decode_v(b >> 8 * j & 0xFF, eb);
-            }
-        }
-        if constexpr (sizeof(TO) == 2) {
-            uint16_t x[4], y[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = f32_to_bf16(m[j]), y[j] = f32_to_bf16(v[j]);
-            store4(mo + r.index + off + at, cnt, x);
-            store4(vo + r.index + off + at, cnt, y);
-        } else {
-            store4(mo + r.index + off + at, cnt, m);
-            store4(vo + r.index + off + at, cnt, v);
-        }
-    }
+    if (left == PIECE)
+        moments_piece<TO, BITS, true>(r, off, left, lane, mo, vo);
+    else
+        moments_piece<TO, BITS, false>(r, off, left, lane, mo, vo);
 }
 
 template <int BITS>
@@ -403,22 +501,23 @@ __global__ __launch_bounds__(256) void adamw_set_moments_kernel(const Rec* __res
         if (k * 256 >= left) return;
         const int at = k * 256 + lane * 4, cnt = left - at;
         float m[4], v[4];
-        load4(mi + r.index + off + at, cnt, m);
-        load4(vi + r.index + off + at, cnt, v);
+        load4(global<float>(mi) + r.index + off + at, cnt, m);
+        load4(global<float>(vi) + r.index + off + at, cnt, v);
         if (BITS == 32) {
-            store4((float*)r.m + off + at, cnt, m);
-            store4((float*)r.v + off + at, cnt, v);
+            store4(global<float>(r.m) + off + at, cnt, m);
+            store4(global<float>(r.v) + off + at, cnt, v);
         } else {
-            uint32_t h[4], eb;
+            uint32_t h[4];
             hash4((uint64_t)(r.index + off + at), s, h);
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = v[j] >= 0.f ? v[j] : __uint_as_float(0x7FC00000u);  // no second moment: as sqrt has it
-            const uint32_t a = encode4_m(m, h, eb);
-            if (lane == 0) r.me[off / QBLOCK + k] = (uint8_t)eb;
-            const uint32_t b = encode4_v(v, h, eb);
-            if (lane == 0) r.ve[off / QBLOCK + k] = (uint8_t)eb;
-            store4b((uint8_t*)r.m + off + at, cnt, a);
-            store4b((uint8_t*)r.v + off + at, cnt, b);
+            const uint32_t a = block_exponent(block_top(m)), b = block_exponent(block_top(v));
+            store4b(global<uint8_t>(r.m) + off + at, cnt, encode4_m(m, a, h));
+            store4b(global<uint8_t>(r.v) + off + at, cnt, encode4_v(v, b, h));
+            if (lane == 0) {
+                global<uint8_t>(r.me)[off / QBLOCK + k] = (uint8_t)a;
+                global<uint8_t>(r.ve)[off / QBLOCK + k] = (uint8_t)b;
+            }
         }
     }
 }
@@ -463,7 +562,7 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(S src, uint32_t items, d
     double acc[4] = {0, 0, 0, 0};
     for (uint32_t i = wave_number(); i < items; i += gridDim.x * 4) {
         int64_t n;
-        const T* g = src.template run<T>(i, n);
+        const GLOBAL T* g = global<T>(src.template run<T>(i, n));
         int64_t at = lane * 4;
         for (; at + 3 * 256 + 4 <= n; at += 1024) {
             float x[4][4];
@@ -513,7 +612,7 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const sr_grad_span* __r
     if (factor == 1.f) return;
     const int lane = threadIdx.x & 63;
     for (uint32_t i = wave_number(); i < items; i += gridDim.x * 4) {
-        T* g = (T*)spans[i].g;
+        GLOBAL T* g = global<T>(spans[i].g);
         const int64_t n = spans[i].n;
         for (int64_t at = lane * 4; at < n; at += 256) {
             const int cnt = n - at < 4 ? (int)(n - at) : 4;
