@@ -378,10 +378,12 @@ typedef struct sr_adamw sr_adamw; /* a list of tensors of one dtype and kind of 
 /* `tensors` is a HOST array, copied.  The tensors must not overlap.  SR_ERR_STATE from the other calls: another device is current. */
 int sr_adamw_create(int dtype, int bits, int count, const sr_adamw_tensor* tensors, sr_adamw** out);
 void sr_adamw_destroy(sr_adamw* list);
-/* One step of all tensors.  grads: device array of `count` device pointers to gradients in the list's dtype (any alignment of
- * their elements).  factor: a device float, or NULL (1).  step: counted from 1, with `hyper`; or scalars != NULL: what sr_adamw_tick
- * wrote (hyper and step are then ignored). */
-int sr_adamw_step(const sr_adamw* list, const sr_adamw_hyper* hyper, int64_t step, const void* scalars, const void* const* grads,
+/* One step of all tensors.  grads: array of `count` device pointers to gradients in the list's dtype (any alignment of their
+ * elements), itself on the device, or (on_host != 0, count <= SR_ADAMW_BY_VALUE) on the HOST: it then travels in the kernel's
+ * arguments.  factor: a device float, or NULL (1).  step: counted from 1, with `hyper`; or scalars != NULL: what sr_adamw_tick wrote
+ * (hyper and step are then ignored). */
+#define SR_ADAMW_BY_VALUE 448
+int sr_adamw_step(const sr_adamw* list, const sr_adamw_hyper* hyper, int64_t step, const void* scalars, const void* const* grads, int on_host,
                   const float* factor, void* stream);
 /* For captured graphs: *step += 1 and the scalars of that step, on the device; lr: a device float, or NULL (hyper->lr).
  * scalars: SR_ADAMW_SCALARS_BYTES. */
@@ -400,11 +402,11 @@ typedef struct {
 } sr_grad_span;
 typedef struct {
     const sr_adamw* list;
-    const void* const* grads;
+    const void* const* grads; /* as for sr_adamw_step */
     const sr_grad_span* spans;
     int64_t nspans;
-    int32_t dtype; /* of the spans */
-    int32_t _pad;
+    int32_t dtype;            /* of the spans */
+    int32_t on_host;          /* of grads */
 } sr_grad_list;
 size_t sr_grad_norm_workspace_bytes(int nlists);
 int sr_grad_norm(int nlists, const sr_grad_list* lists, double max_norm, float* out, void* workspace, size_t workspace_bytes,

@@ -66,10 +66,10 @@ class AdamWHyper(C.Structure):
 
 class GradList(C.Structure):
     _fields_ = [('list', C.c_void_p), ('grads', C.c_void_p), ('spans', C.c_void_p), ('nspans', C.c_int64), ('dtype', C.c_int32),
-                ('_pad', C.c_int32)]
+                ('on_host', C.c_int32)]
 
 
-ADAMW_BLOCK, ADAMW_SCALARS_BYTES, ADAMW_SKIP, GRAD_MAX_LISTS = 256, 64, 1, 64
+ADAMW_BLOCK, ADAMW_SCALARS_BYTES, ADAMW_SKIP, ADAMW_BY_VALUE, GRAD_MAX_LISTS = 256, 64, 1, 448, 64
 
 _SIGS = {
     'sr_strerror': (C.c_char_p, [C.c_int]),
@@ -144,7 +144,7 @@ _SIGS = {
     'sr_rrdbnet_profile_read': (C.c_int, [C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_long)]),
     'sr_adamw_create': (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(AdamWTensor), C.POINTER(C.c_void_p)]),
     'sr_adamw_destroy': (None, [C.c_void_p]),
-    'sr_adamw_step': (C.c_int, [C.c_void_p, C.POINTER(AdamWHyper), C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    'sr_adamw_step': (C.c_int, [C.c_void_p, C.POINTER(AdamWHyper), C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
     'sr_adamw_tick': (C.c_int, [C.POINTER(AdamWHyper), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     'sr_adamw_moments': (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
     'sr_adamw_set_moments': (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),

@@ -52,6 +52,17 @@ struct Piece {
     uint32_t tensor, number;  // the number-th PIECE values of the tensor
 };
 
+// The gradients' addresses: they are new tensors every step, and a kernel cannot follow a host list.  Short lists travel in the
+// kernel's arguments (no copy, no second launch: 28 -> 21 us for a step of 53 tensors), long ones lie on the device.
+struct GradsAt {
+    const void* const* at;
+    __device__ __forceinline__ const void* operator[](uint32_t i) const { return at[i]; }
+};
+struct GradsByValue {
+    const void* at[SR_ADAMW_BY_VALUE];
+    __device__ __forceinline__ const void* operator[](uint32_t i) const { return at[i]; }
+};
+
 struct Scalars {
     float b1, c1, b2, c2, decay, step_size, rbc2, eps, d, cd;
     uint32_t k0, k1;
@@ -382,10 +393,10 @@ __device__ __forceinline__ uint32_t wave_number() {
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * (blockDim.x / 64) + threadIdx.x / 64));
 }
 
-template <typename P, int BITS>
+template <typename P, int BITS, typename G>
 __global__ __launch_bounds__(256) void adamw_step_kernel(const Rec* __restrict__ recs, const Piece* __restrict__ pieces, uint32_t npieces,
-                                                         const void* const* __restrict__ grads, const float* __restrict__ factor_at,
-                                                         const Scalars* __restrict__ scalars_at, Scalars scalars) {
+                                                         const float* __restrict__ factor_at, const Scalars* __restrict__ scalars_at,
+                                                         Scalars scalars, G grads) {
     const uint32_t w = wave_number();
     const int lane = threadIdx.x & 63;
     if (w >= npieces) return;
@@ -525,10 +536,11 @@ __global__ __launch_bounds__(256) void adamw_set_moments_kernel(const Rec* __res
 // ---- global gradient norm ---------------------------------------------------------------------------------------------
 // Squares are added in float64 (a float32 square overflows from 1.8e19 on, and 1e8 of them lose three digits), in an order
 // that the shapes alone determine.  Work items are runs of consecutive values; waves take them in turn.
+template <typename G>
 struct PieceSource {  // the pieces of an optimizer's list, gradients by tensor
     const Rec* recs;
     const Piece* pieces;
-    const void* const* grads;
+    G grads;
     template <typename T>
     __device__ __forceinline__ const T* run(uint32_t i, int64_t& n) const {
         const Piece c = pieces[i];
@@ -729,22 +741,17 @@ extern "C" void sr_adamw_destroy(sr_adamw* l) {
     delete l;
 }
 
-extern "C" int sr_adamw_step(const sr_adamw* l, const sr_adamw_hyper* h, int64_t step, const void* scalars, const void* const* grads,
-                             const float* factor, void* stream) {
-    SR_REQUIRE(l && grads);
-    Scalars s = {};
-    if (!scalars) {
-        const int rc = check_hyper(h, step);
-        if (rc) return rc;
-        s = make_scalars(*h, h->lr, step);
-    }
-    const int rc = on_device(l);
-    if (rc) return rc;
-    if (!l->npieces) return SR_OK;
+namespace {
+GradsByValue by_value(const sr_adamw* l, const void* const* grads) {
+    GradsByValue g;
+    memcpy(g.at, grads, sizeof(void*) * (size_t)l->count);
+    memset(g.at + l->count, 0, sizeof(void*) * (size_t)(SR_ADAMW_BY_VALUE - l->count));
+    return g;
+}
+template <typename G>
+void launch_step(const sr_adamw* l, const G& g, const Scalars* at, const Scalars& s, const float* factor, hipStream_t st) {
     const dim3 grid(waves_to_wgs(l->npieces));
-    hipStream_t st = (hipStream_t)stream;
-    const Scalars* at = (const Scalars*)scalars;
-#define SR_STEP(P, BITS) adamw_step_kernel<P, BITS><<<grid, 256, 0, st>>>(l->recs(), l->pieces(), l->npieces, grads, factor, at, s)
+#define SR_STEP(P, BITS) adamw_step_kernel<P, BITS, G><<<grid, 256, 0, st>>>(l->recs(), l->pieces(), l->npieces, factor, at, s, g)
     if (l->dtype == SR_F32) {
         if (l->bits == 32)
             SR_STEP(float, 32);
@@ -757,6 +764,32 @@ extern "C" int sr_adamw_step(const sr_adamw* l, const sr_adamw_hyper* h, int64_t
             SR_STEP(bf16_t, 8);
     }
 #undef SR_STEP
+}
+template <typename S>
+void launch_norm(int dtype, uint32_t wgs, const S& src, uint32_t items, double* out, hipStream_t st) {
+    if (dtype == SR_F32)
+        grad_norm_kernel<float><<<wgs, 256, 0, st>>>(src, items, out);
+    else
+        grad_norm_kernel<bf16_t><<<wgs, 256, 0, st>>>(src, items, out);
+}
+}  // namespace
+
+extern "C" int sr_adamw_step(const sr_adamw* l, const sr_adamw_hyper* h, int64_t step, const void* scalars, const void* const* grads, int on_host,
+                             const float* factor, void* stream) {
+    SR_REQUIRE(l && grads && (!on_host || l->count <= SR_ADAMW_BY_VALUE));
+    Scalars s = {};
+    if (!scalars) {
+        const int rc = check_hyper(h, step);
+        if (rc) return rc;
+        s = make_scalars(*h, h->lr, step);
+    }
+    const int rc = on_device(l);
+    if (rc) return rc;
+    if (!l->npieces) return SR_OK;
+    if (on_host)
+        launch_step(l, by_value(l, grads), (const Scalars*)scalars, s, factor, (hipStream_t)stream);
+    else
+        launch_step(l, GradsAt{grads}, (const Scalars*)scalars, s, factor, (hipStream_t)stream);
     SR_LAUNCH_CHECK();
     return SR_OK;
 }
@@ -819,7 +852,7 @@ extern "C" int sr_grad_norm(int nlists, const sr_grad_list* lists, double max_no
     for (int i = 0; i < nlists; ++i) {
         const sr_grad_list& l = lists[i];
         if (l.list) {
-            SR_REQUIRE(l.grads);
+            SR_REQUIRE(l.grads && (!l.on_host || l.list->count <= SR_ADAMW_BY_VALUE));
             const int rc = on_device(l.list);
             if (rc) return rc;
         } else {
@@ -838,20 +871,12 @@ extern "C" int sr_grad_norm(int nlists, const sr_grad_list* lists, double max_no
         const uint32_t want = waves_to_wgs(items), wgs = want < NORM_WG ? want : NORM_WG;
         parts.n[i] = (int32_t)wgs;
         double* out_i = (double*)workspace + (size_t)i * NORM_WG;
-        const int dtype = l.list ? l.list->dtype : l.dtype;
-        if (l.list) {
-            const PieceSource src = {l.list->recs(), l.list->pieces(), l.grads};
-            if (dtype == SR_F32)
-                grad_norm_kernel<float><<<wgs, 256, 0, st>>>(src, items, out_i);
-            else
-                grad_norm_kernel<bf16_t><<<wgs, 256, 0, st>>>(src, items, out_i);
-        } else {
-            const SpanSource src = {l.spans};
-            if (dtype == SR_F32)
-                grad_norm_kernel<float><<<wgs, 256, 0, st>>>(src, items, out_i);
-            else
-                grad_norm_kernel<bf16_t><<<wgs, 256, 0, st>>>(src, items, out_i);
-        }
+        if (!l.list)
+            launch_norm(l.dtype, wgs, SpanSource{l.spans}, items, out_i, st);
+        else if (l.on_host)
+            launch_norm(l.list->dtype, wgs, PieceSource<GradsByValue>{l.list->recs(), l.list->pieces(), by_value(l.list, l.grads)}, items, out_i, st);
+        else
+            launch_norm(l.list->dtype, wgs, PieceSource<GradsAt>{l.list->recs(), l.list->pieces(), {l.grads}}, items, out_i, st);
         SR_LAUNCH_CHECK();
     }
     grad_norm_finish_kernel<<<1, 256, 0, st>>>(parts, (const double*)workspace, max_norm, out);

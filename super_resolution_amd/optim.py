@@ -7,6 +7,7 @@ train/train_realESRGAN_fdconv.py:142, and the weight average that Real-ESRGAN ch
 `train.FlatAdam` re-points the parameters into one buffer and runs torch operators on it; `AdamW` leaves them where they are:
 one kernel (csrc/adamw.hip) walks all tensors of a group, reads gradients, parameters and moments once and writes them once.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -17,7 +18,7 @@ from . import _lib as L
 
 _HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libsr_amd_torch.so')
 _host = None
-_BY_VALUE = 4 * 3840   # bytes of a table that go to the device as kernel arguments (four launches); longer ones are copied
+_BY_VALUE = 3840   # bytes of a table that go to the device as kernel arguments, in one launch; longer ones are copied
 
 
 def _host_lib():
@@ -42,19 +43,32 @@ def _host_failed(what):
     raise RuntimeError('%s: %s' % (what, _host_lib().srt_message().decode()))
 
 
-def _upload(nbytes, write, dev):
-    """A table of nbytes on the device; write(address) fills it on the host.  Under capture it travels by value: a copy node would
+def _on(dev):
+    """torch.cuda.device(dev), which takes 2 us, where another device is current."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+class _Stage:
+    """Host memory at `at` for a table of nbytes, and its way to the device.  Under capture it travels by value: a copy node would
     read the host buffer again at every replay."""
-    table = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
-    if nbytes <= _BY_VALUE or torch.cuda.is_current_stream_capturing():
-        buf = (C.c_char * max(nbytes, 1))()
-        write(C.addressof(buf))
-        L.check(L.lib().sr_upload(C.addressof(buf), table.data_ptr(), nbytes, L.stream_ptr(dev)), 'sr_upload')
-    else:
-        stage = torch.empty(nbytes, dtype=torch.uint8, pin_memory=True)
-        write(stage.data_ptr())
-        table.copy_(stage, non_blocking=True)   # torch keeps the pinned block until the copy is done
-    return table
+
+    def __init__(self, nbytes):
+        self.nbytes = nbytes
+        self.by_value = nbytes <= _BY_VALUE or torch.cuda.is_current_stream_capturing()
+        if self.by_value:
+            self.host = (C.c_char * max(nbytes, 1))()
+            self.at = C.addressof(self.host)
+        else:
+            self.host = torch.empty(nbytes, dtype=torch.uint8, pin_memory=True)
+            self.at = self.host.data_ptr()
+
+    def upload(self, dev, st):
+        table = torch.empty(max(self.nbytes, 1), dtype=torch.uint8, device=dev)
+        if self.by_value:
+            L.check(L.lib().sr_upload(self.at, table.data_ptr(), self.nbytes, st), 'sr_upload')
+        else:
+            table.copy_(self.host, non_blocking=True)   # torch keeps the pinned block until the copy is done
+        return table
 
 
 def _exchange_gradients(params, group, average):
@@ -132,19 +146,22 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     if not counts[2]:
         return torch.tensor(0.0)
     dev = torch.device('cuda', device.value)
-    with torch.cuda.device(dev):
+    with _on(dev):
+        st = L.stream_ptr(dev)
         n32, n16 = counts[0], counts[1]
-        spans = _upload(16 * (n32 + n16), host.srt_take_spans, dev)
+        stage = _Stage(16 * (n32 + n16))
+        host.srt_take_spans(stage.at)
+        spans = stage.upload(dev, st)
         lists = (L.GradList * 2)()
         lists[0].spans, lists[0].nspans, lists[0].dtype = spans.data_ptr(), n32, L.SR_F32
         lists[1].spans, lists[1].nspans, lists[1].dtype = spans.data_ptr() + 16 * n32, n16, L.SR_BF16
-        out = _norm(lists, max_norm, dev)
+        buf, at = _norm(lists, max_norm, dev, st)
+        out = buf[at:].view(torch.float32)
         if error_if_nonfinite and not bool(torch.isfinite(out[0])):
             raise RuntimeError('clip_grad_norm_: the norm of the gradients is not finite')
-        factor, st = out.data_ptr() + 4, L.stream_ptr(dev)
         for l in lists:
             if l.nspans:
-                L.check(lib.sr_grad_scale(l.dtype, l.nspans, l.spans, factor, st), 'sr_grad_scale')
+                L.check(lib.sr_grad_scale(l.dtype, l.nspans, l.spans, buf.data_ptr() + at + 4, st), 'sr_grad_scale')
         for g in odd:
             g.mul_(out[1])
     return out[0]
@@ -162,13 +179,14 @@ def _is_dense(t):
     return True
 
 
-def _norm(lists, max_norm, dev):
-    """(norm, factor) as a float32 pair on the device."""
+def _norm(lists, max_norm, dev, st):
+    """(buffer, at): norm and factor as float32 at buffer[at:] (bytes, on the device)."""
     lib, n = L.lib(), len(lists)
-    out = torch.empty(2, dtype=torch.float32, device=dev)
-    ws = torch.empty(lib.sr_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
-    L.check(lib.sr_grad_norm(n, lists, max_norm, out.data_ptr(), ws.data_ptr(), ws.numel(), L.stream_ptr(dev)), 'sr_grad_norm')
-    return out
+    at = lib.sr_grad_norm_workspace_bytes(n)
+    buf = torch.empty(at + 8, dtype=torch.uint8, device=dev)
+    ws = buf.data_ptr()
+    L.check(lib.sr_grad_norm(n, lists, max_norm, ws + at, ws, at, st), 'sr_grad_norm')
+    return buf, at
 
 
 # ------------------------------------------------------------------------------------------------------------------
@@ -185,7 +203,7 @@ class _List:
         self.dtype = self.params[0].dtype
         self.handle, self.tracked, self.retired = None, None, []
         self.steps = 0              # int: all tensors alike; else an int64 array
-        self.ptrs = (C.c_uint64 * self.n)()
+        self.ptrs = self.stage = None
         self.odd = (C.c_int64 * self.n)()
         self.nodd, self.moved = C.c_int64(), C.c_int64()
         self.seen = self.step_dev = self.scalars = None
@@ -233,6 +251,8 @@ class _List:
 
     def gradients(self, keep):
         """Fills self.ptrs; returns the number of tensors without a gradient.  keep: copies that must live until the launch."""
+        self.stage = stage = _Stage(8 * self.n)
+        self.ptrs = (C.c_uint64 * self.n).from_address(stage.at)
         missing = _host_lib().srt_gradients(self.tracked, self.ptrs, self.odd, C.byref(self.nodd), C.byref(self.moved))
         if missing < 0:
             _host_failed('AdamW')
@@ -242,14 +262,22 @@ class _List:
             if g.layout != torch.strided or g.shape != p.shape or g.dtype != p.dtype or g.device != p.device:
                 raise RuntimeError('AdamW: the gradient of parameter %d (%s %s on %s) does not fit it (%s %s on %s)'
                                    % (self.members[self.odd[k]], tuple(g.shape), g.dtype, g.device, tuple(p.shape), p.dtype, p.device))
-            g = torch.empty_like(p).copy_(g)
+            with torch.no_grad():
+                g = torch.empty_like(p).copy_(g)
             keep.append(g)
             self.ptrs[self.odd[k]] = g.data_ptr()
         return missing
 
-    def table(self, dev, ptrs=None):
-        ptrs = self.ptrs if ptrs is None else ptrs
-        return _upload(8 * self.n, lambda at: C.memmove(at, ptrs, 8 * self.n), dev)
+    def table(self, dev, st, ptrs=None):
+        """What the kernels read the gradients' addresses from: (address, whether on the host, what keeps it)."""
+        stage = self.stage
+        if ptrs is not None:
+            stage = _Stage(8 * self.n)
+            C.memmove(stage.at, ptrs, 8 * self.n)
+        if self.n <= L.ADAMW_BY_VALUE:
+            return stage.at, 1, stage
+        t = stage.upload(dev, st)
+        return t.data_ptr(), 0, t
 
 
 class AdamW(torch.optim.Optimizer):
@@ -334,7 +362,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError('AdamW: at most %d parameter groups of one dtype' % L.GRAD_MAX_LISTS)
             for lst in self._lists:
                 lst.build(self)
-        self.grad_norm = None   # of the last step with clip_grad_norm
+        self._norm = None
         self._built = True
 
     def add_param_group(self, param_group):
@@ -368,13 +396,16 @@ class AdamW(torch.optim.Optimizer):
         return L.AdamWHyper(lr, b1, b2, g['eps'], g['weight_decay'], self.ema_decay or 0.0, self.seed)
 
     def _reset_ema(self):
-        for p, at in zip(self.params, self._index):
-            self.ema[at:at + p.numel()].copy_(self._flat(p))
+        if self.numel:
+            self.ema.copy_(self._cat(self.params))
 
     @staticmethod
-    def _flat(t):
-        """A dense tensor's elements in memory order."""
-        return t.detach().as_strided((t.numel(),), (1,))
+    def _cat(tensors):
+        """Dense tensors' elements in memory order, one after the other."""
+        with torch.no_grad():
+            if len({t.dtype for t in tensors}) == 1 and all(t.is_contiguous() for t in tensors):
+                return torch._utils._flatten_dense_tensors(tensors)    # one C++ call for thousands of tensors
+            return torch.cat([t.as_strided((t.numel(),), (1,)).float() for t in tensors])
 
     def _shaped(self, flat, i):
         """Tensor i's part of a flat array, in the parameter's shape and strides."""
@@ -398,7 +429,7 @@ class AdamW(torch.optim.Optimizer):
         """(exp_avg, exp_avg_sq) of all parameters as new flat tensors, in the order of the parameters; 8-bit moments as the values
         that their codes stand for (bfloat16 holds those of m and v exactly, within its range)."""
         code = L.dtype_code(dtype)
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             m, v = (torch.empty(self.numel, dtype=dtype, device=self.device) for _ in range(2))
             for lst in self._lists:
                 if self.numel:
@@ -412,18 +443,19 @@ class AdamW(torch.optim.Optimizer):
         return [self._shaped(self.ema, i) for i in range(len(self.params))]
 
     # ---- step ----------------------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, closure=None, group=None, average=True, clip_grad_norm=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
         if _world(group) > 1:
-            _exchange_gradients(self.params, group, average)
+            with torch.no_grad():
+                _exchange_gradients(self.params, group, average)
         if clip_grad_norm is not None and not clip_grad_norm >= 0:
             raise ValueError('AdamW: clip_grad_norm must not be negative (got %r)' % (clip_grad_norm,))
         dev = self.device
-        with torch.cuda.device(dev):
+        with _on(dev):
+            st = L.stream_ptr(dev)
             capturing = torch.cuda.is_current_stream_capturing()
             if capturing and not self.capturable:
                 raise RuntimeError('AdamW: a step under graph capture needs capturable=True (the step count would stay what it is now)')
@@ -435,25 +467,30 @@ class AdamW(torch.optim.Optimizer):
                     self._follow(lst, capturing)
                 if self.capturable and missing[-1] < lst.n:
                     self._same_gradients(lst)
-            tables = [lst.table(dev) for lst in self._lists]
+            tables = [lst.table(dev, st) for lst in self._lists]
             factor = None
             if clip_grad_norm is not None:
                 lists = (L.GradList * len(self._lists))()
                 for l, lst, table in zip(lists, self._lists, tables):
-                    l.list, l.grads = lst.handle, table.data_ptr()
-                out = _norm(lists, float(clip_grad_norm), dev)
-                self.grad_norm, factor = out[0], out.data_ptr() + 4
+                    l.list, l.grads, l.on_host = lst.handle, table[0], table[1]
+                self._norm = buf, at = _norm(lists, float(clip_grad_norm), dev, st)
+                factor = buf.data_ptr() + at + 4
             for lst, h, miss, table in zip(self._lists, hypers, missing, tables):
-                self._launch(lst, h, miss, table, factor)
+                self._launch(lst, h, miss, table, factor, st)
                 if _host_lib().srt_written(lst.tracked, lst.ptrs if miss else None) < 0:
                     _host_failed('AdamW')
         return loss
 
-    def _launch(self, lst, h, missing, table, factor):
-        lib, st = L.lib(), L.stream_ptr(self.device)
+    @property
+    def grad_norm(self):
+        """The norm of the last step with clip_grad_norm (a 0-d float32 tensor on the GPU), None before one."""
+        return None if self._norm is None else self._norm[0][self._norm[1]:].view(torch.float32)[0]
 
-        def run(step, scalars, grads):
-            L.check(lib.sr_adamw_step(lst.handle, C.byref(h), step, scalars, grads.data_ptr(), factor, st), 'sr_adamw_step')
+    def _launch(self, lst, h, missing, table, factor, st):
+        lib = L.lib()
+
+        def run(step, scalars, table):
+            L.check(lib.sr_adamw_step(lst.handle, C.byref(h), step, scalars, table[0], table[1], factor, st), 'sr_adamw_step')
         if missing == lst.n:
             if self.ema is not None:
                 run(1, None, table)
@@ -479,7 +516,7 @@ class AdamW(torch.optim.Optimizer):
             now = have & (steps == t) | rest
             rest = np.zeros_like(rest)
             part = np.where(now, ptrs, np.uint64(L.ADAMW_SKIP))
-            run(int(t), None, lst.table(self.device, part.ctypes.data))
+            run(int(t), None, lst.table(self.device, st, part.ctypes.data))
         if (steps == steps[0]).all():
             lst.steps = int(steps[0])
 
@@ -502,7 +539,7 @@ class AdamW(torch.optim.Optimizer):
         """One step count on the device serves all tensors of a list."""
         have = np.frombuffer(lst.ptrs, dtype=np.uint64) != 0
         if lst.seen is None:
-            lst.seen = have
+            lst.seen = have.copy()
         elif not np.array_equal(lst.seen, have):
             raise RuntimeError('AdamW(capturable=True): a step must bring gradients for the same parameters as the one before')
 
@@ -558,15 +595,19 @@ class AdamW(torch.optim.Optimizer):
         for mine, hp in zip(self.param_groups, new):
             mine.update(hp)
 
-        def flat(name, i):
+        def part(name, i):
             p, x = self.params[i], state.get(i, {}).get(name)
             if x is None:
-                return torch.zeros(p.numel(), dtype=torch.float32, device=self.device)
-            x = x.detach().to(self.device, torch.float32)
-            return self._flat(x if x.stride() == p.stride() else torch.empty_like(p, dtype=torch.float32).copy_(x))
-        with torch.cuda.device(self.device):
+                return torch.zeros(p.numel(), dtype=torch.float32, device=self.device) if name != 'ema' else p.float()
+            if x.dtype != torch.float32 or x.device != self.device:
+                x = x.to(self.device, torch.float32)
+            return x if x.stride() == p.stride() else torch.empty_like(p, dtype=torch.float32).copy_(x)
+
+        def flat(name):
+            return self._cat([part(name, i) for i in range(len(self.params))])
+        with _on(self.device):
             if self.numel:
-                m, v = (torch.cat([flat(name, i) for i in range(len(self.params))]) for name in ('exp_avg', 'exp_avg_sq'))
+                m, v = flat('exp_avg'), flat('exp_avg_sq')
                 for lst in self._lists:
                     L.check(L.lib().sr_adamw_set_moments(lst.handle, m.data_ptr(), v.data_ptr(), self.seed, L.stream_ptr(self.device)),
                             'sr_adamw_set_moments')
@@ -580,8 +621,5 @@ class AdamW(torch.optim.Optimizer):
                     lst.seen = None
                 else:
                     lst.steps = int(steps[0]) if (steps == steps[0]).all() else steps
-            if self.ema is not None:
-                self._reset_ema()
-                for i, s in state.items():
-                    if 'ema' in s:
-                        self.ema[self._index[i]:self._index[i] + self.params[i].numel()].copy_(flat('ema', i))
+            if self.ema is not None and self.numel:
+                self.ema.copy_(flat('ema'))

@@ -63,7 +63,7 @@ def test_c_entries_refuse_bad_arguments(L):
     assert ok() == ARG
     t[0].ema = None
     h = L.AdamWHyper(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0)
-    assert lib.sr_adamw_step(None, C.byref(h), 1, None, 4096, None, None) == ARG
+    assert lib.sr_adamw_step(None, C.byref(h), 1, None, 4096, 0, None, None) == ARG
     for bad in (dict(lr=-1.0), dict(beta1=1.0), dict(beta2=-0.1), dict(eps=-1.0), dict(weight_decay=-1.0), dict(ema_decay=1.5), dict(lr=float('nan'))):
         b = L.AdamWHyper(1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0)
         for k, x in bad.items():

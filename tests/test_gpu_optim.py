@@ -497,7 +497,7 @@ def test_element_numbers_beyond_32_bits(T):
         g = to_bf16(grads())[0]
         gd = f32(g).bfloat16()
         table = torch.tensor([gd.data_ptr()], device='cuda')
-        L.check(L.lib().sr_adamw_step(h, C.byref(hyper), step, None, table.data_ptr(), None, L.stream_ptr(par.device)))
+        L.check(L.lib().sr_adamw_step(h, C.byref(hyper), step, None, table.data_ptr(), 0, None, L.stream_ptr(par.device)))
         torch.cuda.synchronize()
         ref.step([g])
         same(par, ref.p[0], 'p, step %d' % step)
