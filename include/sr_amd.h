@@ -394,8 +394,10 @@ int sr_adamw_moments(const sr_adamw* list, int dtype, void* m, void* v, void* st
 int sr_adamw_set_moments(const sr_adamw* list, const float* m, const float* v, uint64_t seed, void* stream);
 
 /* out[0] = sqrt(sum of squares) over all lists (summed in float64 in a fixed order), out[1] = min(1, max_norm / (out[0] + 1e-6)).
- * A list is an sr_adamw with its gradient table, or (list == NULL) a device array of spans; `lists` is a HOST array. */
+ * A list is an sr_adamw with its gradient table, or (list == NULL) an array of spans; `lists` is a HOST array, the arrays that it
+ * points to lie on the device, or with on_host on the HOST (at most SR_ADAMW_BY_VALUE tensors or SR_GRAD_SPANS_BY_VALUE spans). */
 #define SR_GRAD_MAX_LISTS 64
+#define SR_GRAD_SPANS_BY_VALUE 224
 typedef struct {
     void* g; /* n gradients */
     int64_t n;
@@ -406,13 +408,14 @@ typedef struct {
     const sr_grad_span* spans;
     int64_t nspans;
     int32_t dtype;            /* of the spans */
-    int32_t on_host;          /* of grads */
+    int32_t on_host;          /* grads or spans */
 } sr_grad_list;
 size_t sr_grad_norm_workspace_bytes(int nlists);
 int sr_grad_norm(int nlists, const sr_grad_list* lists, double max_norm, float* out, void* workspace, size_t workspace_bytes,
                  void* stream);
-/* g *= *factor over device spans that do not overlap (one wave takes a span at a time: split long tensors) */
-int sr_grad_scale(int dtype, int64_t nspans, const sr_grad_span* spans, const float* factor, void* stream);
+/* g *= *factor over spans that do not overlap (one wave takes a span at a time: split long tensors); nothing is written where
+ * *factor is 1 */
+int sr_grad_scale(int dtype, int64_t nspans, const sr_grad_span* spans, int on_host, const float* factor, void* stream);
 /* Copies a small HOST array (tables of pointers) to the device through kernel arguments: by value, so the source may be reused at
  * once and a captured graph keeps what it held; 3840 bytes per launch.  bytes and dst: multiples of 4. */
 int sr_upload(const void* src_host, void* dst, size_t bytes, void* stream);

@@ -552,12 +552,22 @@ struct PieceSource {  // the pieces of an optimizer's list, gradients by tensor
         return g + off;
     }
 };
+struct SpansAt {
+    const sr_grad_span* at;
+    __device__ __forceinline__ sr_grad_span operator[](uint32_t i) const { return at[i]; }
+};
+struct SpansByValue {
+    sr_grad_span at[SR_GRAD_SPANS_BY_VALUE];
+    __device__ __forceinline__ sr_grad_span operator[](uint32_t i) const { return at[i]; }
+};
+template <typename S>
 struct SpanSource {
-    const sr_grad_span* spans;
+    S spans;
     template <typename T>
     __device__ __forceinline__ const T* run(uint32_t i, int64_t& n) const {
-        n = spans[i].n;
-        return (const T*)spans[i].g;
+        const sr_grad_span s = spans[i];
+        n = s.n;
+        return (const T*)s.g;
     }
 };
 
@@ -567,29 +577,73 @@ __device__ __forceinline__ double wave_sum(double x) {
     return x;
 }
 
+// 16 bytes of gradients
+template <typename T>
+constexpr int W16 = 16 / (int)sizeof(T);
+typedef uint32_t w4u __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void load16(const GLOBAL float* p, float (&x)[4]) { load4(p, 4, x); }
+__device__ __forceinline__ void load16(const GLOBAL bf16_t* p, float (&x)[8]) {
+    const w4u w = *(const GLOBAL w4u*)p;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[2 * j] = lo_f(w[j]), x[2 * j + 1] = hi_f(w[j]);
+}
+__device__ __forceinline__ void store16(GLOBAL float* p, const float (&x)[4]) { store4(p, 4, x); }
+__device__ __forceinline__ void store16(GLOBAL bf16_t* p, const float (&x)[8]) {
+    w4u w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = pack2(x[2 * j], x[2 * j + 1]);
+    *(GLOBAL w4u*)p = w;
+}
+
+// U loads in flight, as long as there are U more for every lane
+template <int U, typename T>
+__device__ __forceinline__ void add_squares(const GLOBAL T* g, int64_t& at, int64_t whole, double (&acc)[4]) {
+    constexpr int W = W16<T>;
+    for (; at + (U - 1) * 64 * W < whole; at += U * 64 * W) {
+        float x[U][W];
+#pragma unroll
+        for (int k = 0; k < U; ++k) load16(g + at + k * 64 * W, x[k]);
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+            for (int j = 0; j < W; ++j) acc[j & 3] = fma((double)x[k][j], (double)x[k][j], acc[j & 3]);
+    }
+}
+template <int U, typename T>
+__device__ __forceinline__ void scale_by(GLOBAL T* g, int64_t& at, int64_t whole, float factor) {
+    constexpr int W = W16<T>;
+    for (; at + (U - 1) * 64 * W < whole; at += U * 64 * W) {
+        float x[U][W];
+#pragma unroll
+        for (int k = 0; k < U; ++k) load16(g + at + k * 64 * W, x[k]);
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) x[k][j] *= factor;
+            store16(g + at + k * 64 * W, x[k]);
+        }
+    }
+}
+
 template <typename T, typename S>
 __global__ __launch_bounds__(256) void grad_norm_kernel(S src, uint32_t items, double* __restrict__ partial) {
+    constexpr int W = W16<T>;
     __shared__ double sums[4];
     const int lane = threadIdx.x & 63;
     double acc[4] = {0, 0, 0, 0};
     for (uint32_t i = wave_number(); i < items; i += gridDim.x * 4) {
         int64_t n;
         const GLOBAL T* g = global<T>(src.template run<T>(i, n));
-        int64_t at = lane * 4;
-        for (; at + 3 * 256 + 4 <= n; at += 1024) {
-            float x[4][4];
+        const int64_t whole = n / (64 * W) * (64 * W);  // full loads of all lanes
+        int64_t at = lane * W;
+        add_squares<4>(g, at, whole, acc);
+        add_squares<2>(g, at, whole, acc);
+        add_squares<1>(g, at, whole, acc);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) load4(g + at + k * 256, 4, x[k]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j] = fma((double)x[k][j], (double)x[k][j], acc[j]);
-        }
-        for (; at < n; at += 256) {
-            float x[4];
-            load4(g + at, n - at < 4 ? (int)(n - at) : 4, x);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = fma((double)x[j], (double)x[j], acc[j]);
+        for (int k = 0; k < W; ++k) {  // what is left, one value a lane
+            const int64_t rest = whole + k * 64 + lane;
+            const float x = rest < n ? Elem<T>::ld((const T*)(g + rest)) : 0.f;
+            acc[k & 3] = fma((double)x, (double)x, acc[k & 3]);
         }
     }
     const double sum = wave_sum((acc[0] + acc[1]) + (acc[2] + acc[3]));
@@ -618,28 +672,24 @@ __global__ __launch_bounds__(256) void grad_norm_finish_kernel(Partials parts, c
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void grad_scale_kernel(const sr_grad_span* __restrict__ spans, uint32_t items, const float* __restrict__ factor_at) {
+template <typename T, typename S>
+__global__ __launch_bounds__(256) void grad_scale_kernel(S spans, uint32_t items, const float* __restrict__ factor_at) {
+    constexpr int W = W16<T>;
     const float factor = *factor_at;
     if (factor == 1.f) return;
     const int lane = threadIdx.x & 63;
     for (uint32_t i = wave_number(); i < items; i += gridDim.x * 4) {
-        GLOBAL T* g = global<T>(spans[i].g);
-        const int64_t n = spans[i].n;
-        for (int64_t at = lane * 4; at < n; at += 256) {
-            const int cnt = n - at < 4 ? (int)(n - at) : 4;
-            float x[4];
-            load4(g + at, cnt, x);
-            if constexpr (sizeof(T) == 2) {
-                uint16_t y[4];
+        const sr_grad_span span = spans[i];
+        GLOBAL T* g = global<T>(span.g);
+        const int64_t n = span.n, whole = n / (64 * W) * (64 * W);
+        int64_t at = lane * W;
+        scale_by<4>(g, at, whole, factor);
+        scale_by<2>(g, at, whole, factor);
+        scale_by<1>(g, at, whole, factor);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = f32_to_bf16(x[j] * factor);
-                store4(g + at, cnt, y);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] *= factor;
-                store4(g + at, cnt, x);
-            }
+        for (int k = 0; k < W; ++k) {
+            const int64_t rest = whole + k * 64 + lane;
+            if (rest < n) Elem<T>::st((T*)(g + rest), Elem<T>::ld((const T*)(g + rest)) * factor);
         }
     }
 }
@@ -765,6 +815,19 @@ void launch_step(const sr_adamw* l, const G& g, const Scalars* at, const Scalars
     }
 #undef SR_STEP
 }
+SpansByValue by_value(const sr_grad_span* spans, int64_t n) {
+    SpansByValue s;
+    memset(&s, 0, sizeof(s));
+    memcpy(s.at, spans, sizeof(sr_grad_span) * (size_t)n);
+    return s;
+}
+template <typename S>
+void launch_scale(int dtype, uint32_t wgs, const S& spans, uint32_t items, const float* factor, hipStream_t st) {
+    if (dtype == SR_F32)
+        grad_scale_kernel<float><<<wgs, 256, 0, st>>>(spans, items, factor);
+    else
+        grad_scale_kernel<bf16_t><<<wgs, 256, 0, st>>>(spans, items, factor);
+}
 template <typename S>
 void launch_norm(int dtype, uint32_t wgs, const S& src, uint32_t items, double* out, hipStream_t st) {
     if (dtype == SR_F32)
@@ -856,7 +919,8 @@ extern "C" int sr_grad_norm(int nlists, const sr_grad_list* lists, double max_no
             const int rc = on_device(l.list);
             if (rc) return rc;
         } else {
-            SR_REQUIRE((l.dtype == SR_F32 || l.dtype == SR_BF16) && l.nspans >= 0 && l.nspans <= 0x7FFFFFFF && (l.spans || !l.nspans));
+            SR_REQUIRE((l.dtype == SR_F32 || l.dtype == SR_BF16) && l.nspans >= 0 && l.nspans <= (l.on_host ? SR_GRAD_SPANS_BY_VALUE : 0x7FFFFFFF) &&
+                       (l.spans || !l.nspans));
         }
     }
     if (nlists && (!workspace || workspace_bytes < sr_grad_norm_workspace_bytes(nlists))) return SR_ERR_WORKSPACE;
@@ -871,8 +935,10 @@ extern "C" int sr_grad_norm(int nlists, const sr_grad_list* lists, double max_no
         const uint32_t want = waves_to_wgs(items), wgs = want < NORM_WG ? want : NORM_WG;
         parts.n[i] = (int32_t)wgs;
         double* out_i = (double*)workspace + (size_t)i * NORM_WG;
-        if (!l.list)
-            launch_norm(l.dtype, wgs, SpanSource{l.spans}, items, out_i, st);
+        if (!l.list && l.on_host)
+            launch_norm(l.dtype, wgs, SpanSource<SpansByValue>{by_value(l.spans, l.nspans)}, items, out_i, st);
+        else if (!l.list)
+            launch_norm(l.dtype, wgs, SpanSource<SpansAt>{{l.spans}}, items, out_i, st);
         else if (l.on_host)
             launch_norm(l.list->dtype, wgs, PieceSource<GradsByValue>{l.list->recs(), l.list->pieces(), by_value(l.list, l.grads)}, items, out_i, st);
         else
@@ -884,14 +950,15 @@ extern "C" int sr_grad_norm(int nlists, const sr_grad_list* lists, double max_no
     return SR_OK;
 }
 
-extern "C" int sr_grad_scale(int dtype, int64_t nspans, const sr_grad_span* spans, const float* factor, void* stream) {
-    SR_REQUIRE((dtype == SR_F32 || dtype == SR_BF16) && nspans >= 0 && nspans <= 0x7FFFFFFF && (spans || !nspans) && factor);
+extern "C" int sr_grad_scale(int dtype, int64_t nspans, const sr_grad_span* spans, int on_host, const float* factor, void* stream) {
+    SR_REQUIRE((dtype == SR_F32 || dtype == SR_BF16) && nspans >= 0 && nspans <= (on_host ? SR_GRAD_SPANS_BY_VALUE : 0x7FFFFFFF));
+    SR_REQUIRE((spans || !nspans) && factor);
     if (!nspans) return SR_OK;
     const uint32_t want = waves_to_wgs((uint32_t)nspans), wgs = want < NORM_WG ? want : NORM_WG;
-    if (dtype == SR_F32)
-        grad_scale_kernel<float><<<wgs, 256, 0, (hipStream_t)stream>>>(spans, (uint32_t)nspans, factor);
+    if (on_host)
+        launch_scale(dtype, wgs, by_value(spans, nspans), (uint32_t)nspans, factor, (hipStream_t)stream);
     else
-        grad_scale_kernel<bf16_t><<<wgs, 256, 0, (hipStream_t)stream>>>(spans, (uint32_t)nspans, factor);
+        launch_scale(dtype, wgs, SpansAt{spans}, (uint32_t)nspans, factor, (hipStream_t)stream);
     SR_LAUNCH_CHECK();
     return SR_OK;
 }

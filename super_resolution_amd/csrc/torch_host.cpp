@@ -91,7 +91,8 @@ SRT_API void srt_untrack(void* h) { delete (Tracked*)h; }
 
 // out[i] = address of the gradient of tensor i, 0 without one.  Returns the number of tensors without a gradient.
 // odd[0 .. *nodd): tensors whose gradient cannot be read as it lies (other shape, strides, dtype or device: out[i] = 0, not counted
-// as missing).  *moved: tensors that are not where, or what, they were when the list was made.
+// as missing).  Tensors with a gradient are about to be written in place: their version counters move (autograd's saved-tensor checks
+// and caches keyed on them must see it; here and not in a walk of its own, which costs as much again).  *moved: tensors that are not where, or what, they were when the list was made.
 SRT_API int64_t srt_gradients(void* h, uint64_t* out, int64_t* odd, int64_t* nodd, int64_t* moved) {
     return guarded([&]() -> int64_t {
         const Tracked& t = *(const Tracked*)h;
@@ -108,6 +109,7 @@ SRT_API int64_t srt_gradients(void* h, uint64_t* out, int64_t* odd, int64_t* nod
                 ++missing;
                 continue;
             }
+            if (!p->is_inference()) p->bump_version();
             const c10::TensorImpl* g = grad->unsafeGetTensorImpl();
             // (equal key sets: the same kind of tensor on the same kind of device)
             if (g->key_set() == p->key_set() && g->numel() == was.numel && g->dtype() == was.dtype && g->device() == was.device && same_layout(g, p))
@@ -116,17 +118,6 @@ SRT_API int64_t srt_gradients(void* h, uint64_t* out, int64_t* odd, int64_t* nod
                 odd[(*nodd)++] = (int64_t)i;
         }
         return missing;
-    });
-}
-
-// the tensors were written in place (autograd's saved-tensor checks and caches keyed on the version must see it);
-// skip != NULL: only where skip[i] != 0
-SRT_API int64_t srt_written(void* h, const uint64_t* skip) {
-    return guarded([&]() -> int64_t {
-        const Tracked& t = *(const Tracked*)h;
-        for (size_t i = 0; i < t.params.size(); ++i)
-            if (!skip || skip[i]) t.params[i].unsafeGetTensorImpl()->bump_version();
-        return 0;
     });
 }
 

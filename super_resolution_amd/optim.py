@@ -32,7 +32,6 @@ def _host_lib():
         h.srt_track.restype, h.srt_track.argtypes = C.c_void_p, [C.py_object]
         h.srt_untrack.restype, h.srt_untrack.argtypes = None, [C.c_void_p]
         h.srt_gradients.restype, h.srt_gradients.argtypes = C.c_int64, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
-        h.srt_written.restype, h.srt_written.argtypes = C.c_int64, [C.c_void_p, C.c_void_p]
         h.srt_spans.restype, h.srt_spans.argtypes = C.c_int64, [C.py_object, C.c_int, C.c_void_p, C.c_void_p]
         h.srt_take_spans.restype, h.srt_take_spans.argtypes = None, [C.c_void_p]
         _host = h
@@ -151,20 +150,21 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
         n32, n16 = counts[0], counts[1]
         stage = _Stage(16 * (n32 + n16))
         host.srt_take_spans(stage.at)
-        spans = stage.upload(dev, st)
-        lists = (L.GradList * 2)()
-        lists[0].spans, lists[0].nspans, lists[0].dtype = spans.data_ptr(), n32, L.SR_F32
-        lists[1].spans, lists[1].nspans, lists[1].dtype = spans.data_ptr() + 16 * n32, n16, L.SR_BF16
-        buf, at = _norm(lists, max_norm, dev, st)
-        out = buf[at:].view(torch.float32)
-        if error_if_nonfinite and not bool(torch.isfinite(out[0])):
+        on_host = int(n32 + n16 <= L.GRAD_SPANS_BY_VALUE)
+        spans = stage.at if on_host else stage.upload(dev, st)
+        first = spans if on_host else spans.data_ptr()
+        lists = (L.GradList * (1 + (n16 > 0 and n32 > 0)))()
+        for l, (at, n, code) in zip(lists, [x for x in ((first, n32, L.SR_F32), (first + 16 * n32, n16, L.SR_BF16)) if x[1]]):
+            l.spans, l.nspans, l.dtype, l.on_host = at, n, code, on_host
+        buf, norm = _norm(lists, max_norm, dev, st)
+        if error_if_nonfinite and not bool(torch.isfinite(norm)):
             raise RuntimeError('clip_grad_norm_: the norm of the gradients is not finite')
         for l in lists:
             if l.nspans:
-                L.check(lib.sr_grad_scale(l.dtype, l.nspans, l.spans, buf.data_ptr() + at + 4, st), 'sr_grad_scale')
+                L.check(lib.sr_grad_scale(l.dtype, l.nspans, l.spans, l.on_host, buf.data_ptr() + 4 * buf.numel() - 4, st), 'sr_grad_scale')
         for g in odd:
-            g.mul_(out[1])
-    return out[0]
+            g.mul_(buf[-1])
+    return norm
 
 
 def _is_dense(t):
@@ -180,13 +180,13 @@ def _is_dense(t):
 
 
 def _norm(lists, max_norm, dev, st):
-    """(buffer, at): norm and factor as float32 at buffer[at:] (bytes, on the device)."""
+    """(a float32 buffer on the device whose last two elements are norm and factor, the norm)."""
     lib, n = L.lib(), len(lists)
-    at = lib.sr_grad_norm_workspace_bytes(n)
-    buf = torch.empty(at + 8, dtype=torch.uint8, device=dev)
+    nbytes = lib.sr_grad_norm_workspace_bytes(n)
+    buf = torch.empty(nbytes // 4 + 2, dtype=torch.float32, device=dev)
     ws = buf.data_ptr()
-    L.check(lib.sr_grad_norm(n, lists, max_norm, ws + at, ws, at, st), 'sr_grad_norm')
-    return buf, at
+    L.check(lib.sr_grad_norm(n, lists, max_norm, ws + nbytes, ws, nbytes, st), 'sr_grad_norm')
+    return buf, buf[-2]
 
 
 # ------------------------------------------------------------------------------------------------------------------
@@ -362,7 +362,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError('AdamW: at most %d parameter groups of one dtype' % L.GRAD_MAX_LISTS)
             for lst in self._lists:
                 lst.build(self)
-        self._norm = None
+        self.grad_norm = None   # of the last step with clip_grad_norm: a 0-d float32 tensor on the GPU
         self._built = True
 
     def add_param_group(self, param_group):
@@ -473,18 +473,11 @@ class AdamW(torch.optim.Optimizer):
                 lists = (L.GradList * len(self._lists))()
                 for l, lst, table in zip(lists, self._lists, tables):
                     l.list, l.grads, l.on_host = lst.handle, table[0], table[1]
-                self._norm = buf, at = _norm(lists, float(clip_grad_norm), dev, st)
-                factor = buf.data_ptr() + at + 4
+                buf, self.grad_norm = _norm(lists, float(clip_grad_norm), dev, st)
+                factor = buf.data_ptr() + 4 * buf.numel() - 4
             for lst, h, miss, table in zip(self._lists, hypers, missing, tables):
                 self._launch(lst, h, miss, table, factor, st)
-                if _host_lib().srt_written(lst.tracked, lst.ptrs if miss else None) < 0:
-                    _host_failed('AdamW')
         return loss
-
-    @property
-    def grad_norm(self):
-        """The norm of the last step with clip_grad_norm (a 0-d float32 tensor on the GPU), None before one."""
-        return None if self._norm is None else self._norm[0][self._norm[1]:].view(torch.float32)[0]
 
     def _launch(self, lst, h, missing, table, factor, st):
         lib = L.lib()

@@ -33,12 +33,13 @@ def host(L):
 
 def test_structs_match_the_header(L):
     src = '#include <stdio.h>\n#include "sr_amd.h"\nint main(){printf("%zu %zu %zu %zu %d %d %d\\n", sizeof(sr_adamw_tensor), ' \
-          'sizeof(sr_adamw_hyper), sizeof(sr_grad_list), sizeof(sr_grad_span), SR_ADAMW_BLOCK, SR_ADAMW_SCALARS_BYTES, SR_GRAD_MAX_LISTS);return 0;}\n'
+          'sizeof(sr_adamw_hyper), sizeof(sr_grad_list), sizeof(sr_grad_span), SR_ADAMW_BLOCK, SR_ADAMW_SCALARS_BYTES, SR_GRAD_MAX_LISTS);printf("%d %d\\n", SR_ADAMW_BY_VALUE, SR_GRAD_SPANS_BY_VALUE);return 0;}\n'
     with tempfile.TemporaryDirectory() as d:
         open(os.path.join(d, 'a.c'), 'w').write(src)
         subprocess.check_call(['gcc', '-I', os.path.join(ROOT, 'include'), os.path.join(d, 'a.c'), '-o', os.path.join(d, 'a')])
         got = [int(x) for x in subprocess.check_output([os.path.join(d, 'a')]).split()]
-    assert got == [C.sizeof(L.AdamWTensor), C.sizeof(L.AdamWHyper), C.sizeof(L.GradList), 16, L.ADAMW_BLOCK, L.ADAMW_SCALARS_BYTES, L.GRAD_MAX_LISTS]
+    assert got == [C.sizeof(L.AdamWTensor), C.sizeof(L.AdamWHyper), C.sizeof(L.GradList), 16, L.ADAMW_BLOCK, L.ADAMW_SCALARS_BYTES, L.GRAD_MAX_LISTS,
+                   L.ADAMW_BY_VALUE, L.GRAD_SPANS_BY_VALUE]
 
 
 def test_c_entries_refuse_bad_arguments(L):
@@ -83,9 +84,12 @@ def test_c_entries_refuse_bad_arguments(L):
     assert lib.sr_grad_norm(65, lists, 1.0, 4096, 4096, 1 << 30, None) == ARG
     lists[0].dtype = 2
     assert lib.sr_grad_norm(1, lists, 1.0, 4096, 4096, need, None) == ARG
-    assert lib.sr_grad_scale(2, 1, 4096, 4096, None) == ARG and lib.sr_grad_scale(0, -1, 4096, 4096, None) == ARG
-    assert lib.sr_grad_scale(0, 1, None, 4096, None) == ARG and lib.sr_grad_scale(0, 1, 4096, None, None) == ARG
-    assert lib.sr_grad_scale(0, 0, None, 4096, None) == 0
+    lists[0].dtype, lists[0].on_host, lists[0].nspans = 0, 1, L.GRAD_SPANS_BY_VALUE + 1
+    assert lib.sr_grad_norm(1, lists, 1.0, 4096, 4096, need, None) == ARG
+    assert lib.sr_grad_scale(2, 1, 4096, 0, 4096, None) == ARG and lib.sr_grad_scale(0, -1, 4096, 0, 4096, None) == ARG
+    assert lib.sr_grad_scale(0, 1, None, 0, 4096, None) == ARG and lib.sr_grad_scale(0, 1, 4096, 0, None, None) == ARG
+    assert lib.sr_grad_scale(0, L.GRAD_SPANS_BY_VALUE + 1, 4096, 1, 4096, None) == ARG
+    assert lib.sr_grad_scale(0, 0, None, 0, 4096, None) == 0
     assert lib.sr_upload(4096, 4096, 6, None) == ARG and lib.sr_upload(None, 4096, 8, None) == ARG and lib.sr_upload(4096, 4098, 8, None) == ARG
     assert lib.sr_upload(None, None, 0, None) == 0
 
@@ -143,11 +147,8 @@ def test_walk_over_gradients(host):
     ps[4].grad = torch.ones(6, 4).t()
     assert run() == 1 and sorted(odd[:nodd.value]) == [2, 4]
     before = [p._version for p in ps]
-    mask = (C.c_uint64 * len(ps))(*([0, 1] * 3))
-    assert host.srt_written(h, mask) == 0
-    assert [p._version - b for p, b in zip(ps, before)] == [0, 1] * 3
-    assert host.srt_written(h, None) == 0
-    assert [p._version - b for p, b in zip(ps, before)] == [1, 2] * 3
+    run()
+    assert [p._version - b for p, b in zip(ps, before)] == [0, 1, 1, 1, 1, 1]   # those with a gradient are about to be written
     ps[5].data = torch.zeros(1)
     run()
     assert moved.value == 1
