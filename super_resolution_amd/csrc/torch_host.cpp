@@ -51,8 +51,9 @@ struct Span {
     uint64_t g;
     int64_t n;
 };
-std::vector<Span> g_found[2];  // the gradients that the last srt_spans found: float32, bfloat16 (guarded by the GIL)
-int64_t g_longest = 1;
+// the gradients that this thread's last srt_spans found: float32, bfloat16 (another thread may run between it and srt_take_spans)
+thread_local std::vector<Span> g_found[2];
+thread_local int64_t g_longest = 1;
 
 // autograd's part of a tensor, where its gradient is; NULL: none
 const at::Tensor* gradient_of(const c10::TensorImpl* t) {
@@ -91,8 +92,9 @@ SRT_API void srt_untrack(void* h) { delete (Tracked*)h; }
 
 // out[i] = address of the gradient of tensor i, 0 without one.  Returns the number of tensors without a gradient.
 // odd[0 .. *nodd): tensors whose gradient cannot be read as it lies (other shape, strides, dtype or device: out[i] = 0, not counted
-// as missing).  Tensors with a gradient are about to be written in place: their version counters move (autograd's saved-tensor checks
-// and caches keyed on them must see it; here and not in a walk of its own, which costs as much again).  *moved: tensors that are not where, or what, they were when the list was made.
+// as missing).  *moved: tensors that are not where, or what, they were when the list was made.  Tensors with a gradient are about
+// to be written in place: their version counters move (autograd's saved-tensor checks and caches keyed on them must see it; here
+// and not in a walk of its own, which costs a third as much again).
 SRT_API int64_t srt_gradients(void* h, uint64_t* out, int64_t* odd, int64_t* nodd, int64_t* moved) {
     return guarded([&]() -> int64_t {
         const Tracked& t = *(const Tracked*)h;

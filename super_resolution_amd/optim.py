@@ -585,6 +585,9 @@ class AdamW(torch.optim.Optimizer):
         new = [{k: g.get(k, mine[k]) for k in ('lr', 'betas', 'eps', 'weight_decay')} for g, mine in zip(groups, self.param_groups)]
         for hp in new:
             self._hyper(hp)
+        steps = [np.array([int(float(state.get(i, {}).get('step', 0))) for i in lst.members], dtype=np.int64) for lst in self._lists]
+        if self.capturable and any(set(t.tolist()) - {0, int(t.max())} for t in steps):
+            raise ValueError('AdamW.load_state_dict: capturable=True takes one step count')
         for mine, hp in zip(self.param_groups, new):
             mine.update(hp)
 
@@ -604,15 +607,11 @@ class AdamW(torch.optim.Optimizer):
                 for lst in self._lists:
                     L.check(L.lib().sr_adamw_set_moments(lst.handle, m.data_ptr(), v.data_ptr(), self.seed, L.stream_ptr(self.device)),
                             'sr_adamw_set_moments')
-            for lst in self._lists:
-                steps = np.array([int(float(state.get(i, {}).get('step', 0))) for i in lst.members], dtype=np.int64)
+            for lst, t in zip(self._lists, steps):
                 if self.capturable:
-                    t = int(steps.max())
-                    if not all(k in (0, t) for k in steps.tolist()):
-                        raise ValueError('AdamW.load_state_dict: capturable=True takes one step count')
-                    lst.step_dev.fill_(t)
+                    lst.step_dev.fill_(int(t.max()))
                     lst.seen = None
                 else:
-                    lst.steps = int(steps[0]) if (steps == steps[0]).all() else steps
+                    lst.steps = int(t[0]) if (t == t[0]).all() else t
             if self.ema is not None and self.numel:
                 self.ema.copy_(flat('ema'))

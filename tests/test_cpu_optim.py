@@ -211,3 +211,42 @@ def test_reference_matches_torch_adamw():
         opt.step()
     assert np.abs(r.p[0] - t.detach().numpy()).max() <= 5 * 16 * 2 ** -24 * max(1.0, np.abs(p).max())
     assert copy.copy(r.t) == [5]
+
+
+def _exchange_worker(rank, world, port, q):
+    import sys
+    sys.path.insert(0, ROOT)
+    os.environ.update(MASTER_ADDR='127.0.0.1', MASTER_PORT=str(port))
+    import torch.distributed as dist
+    dist.init_process_group('gloo', rank=rank, world_size=world)
+    from super_resolution_amd import optim
+    params = [nn.Parameter(torch.full((3, 2), 1.0 + rank)), nn.Parameter(torch.full((5,), 2.0 + rank)), nn.Parameter(torch.full((4,), 3.0 + rank).bfloat16())]
+    with torch.no_grad():
+        optim._broadcast_parameters(params, None)
+    ok = all(bool((p == v).all()) for p, v in zip(params, (1.0, 2.0, 3.0))) and optim._world(None) == 2
+    params[0].grad = torch.full((3, 2), 1.0 + 2 * rank)
+    params[2].grad = torch.full((4,), 4.0 * rank).bfloat16()
+    if rank == 0:
+        params[1].grad = torch.full((5,), 6.0)       # the other rank has none: zeros
+    optim._exchange_gradients(params, None, True)
+    ok = ok and all(bool((p.grad == v).all()) for p, v in zip(params, (2.0, 3.0, 2.0)))
+    optim._exchange_gradients(params, None, False)
+    ok = ok and all(bool((p.grad == v).all()) for p, v in zip(params, (4.0, 6.0, 4.0)))
+    q.put((rank, ok))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_gradients_and_parameters_over_two_ranks(L):
+    import torch.multiprocessing as mp
+    ctx = mp.get_context('spawn')
+    q = ctx.Queue()
+    port = 33500 + os.getpid() % 2000
+    procs = [ctx.Process(target=_exchange_worker, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    res = sorted(q.get(timeout=120) for _ in procs)
+    for p in procs:
+        p.join(60)
+        assert p.exitcode == 0
+    assert res == [(0, True), (1, True)]

@@ -359,6 +359,77 @@ def test_checkpoints_go_between_torch_and_32_and_8_bits(T):
         copy.deepcopy(dopt)
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('scale,eps', [(1e-25, 1e-8), (1e-18, 1e-8), (1e-18, 1e-13), (1e-9, 0.0), (1.0, 0.0), (1e5, 1e-8), (2e7, 1e-8), (1e9, 1e-8), (1e15, 1e-8)])
+def test_the_ends_of_the_range_bit_for_bit(T, bits, scale, eps):
+    """Gradients whose squares are subnormal or vanish, moments around the bounds between which the kernel leaves out the handling of the
+    range (v 2^60, m 2^20, eps 2^-40), zero gradients with eps 0 (0 / 0, as the formula has it)."""
+    hp = dict(HP, eps=eps)
+    arrays, grads = inputs([2000, 300], 45, scale)
+    params = [nn.Parameter(f32(a)) for a in arrays]
+    opt = T.AdamW(params, state_bits=bits, **hp)
+    ref = R.Tensors(arrays, hp, bits)
+    for step in range(3):
+        gs = grads()
+        for p, g in zip(params, gs):
+            p.grad = f32(g)
+        opt.step()
+        ref.step(gs)
+        m, v = opt.moments()
+        same(m, np.concatenate(ref.m), 'm, step %d' % step)
+        same(v, np.concatenate(ref.v), 'v, step %d' % step)
+        for i, p in enumerate(params):
+            same(p, ref.p[i], 'p[%d], step %d' % (i, step))
+
+
+def test_only_empty_parameters_and_sparse_gradients(T):
+    p = [nn.Parameter(torch.zeros(0, 3, device='cuda')) for _ in range(2)]
+    opt = T.AdamW(p, state_bits=8, ema_decay=0.9)
+    for q in p:
+        q.grad = torch.zeros_like(q)
+    opt.step(clip_grad_norm=1.0)
+    assert float(opt.grad_norm) == 0.0 and opt.moments()[0].numel() == 0 and float(T.clip_grad_norm_(p, 1.0)) == 0.0
+    opt.load_state_dict(opt.state_dict())
+    emb = nn.Embedding(10, 4, sparse=True).cuda()
+    emb(torch.tensor([1, 2], device='cuda')).sum().backward()
+    before = emb.weight.detach().clone()
+    with pytest.raises(RuntimeError, match='does not fit'):
+        T.AdamW(emb.parameters()).step()
+    with pytest.raises(TypeError):
+        T.clip_grad_norm_(emb.parameters(), 1.0)
+    assert torch.equal(emb.weight, before)
+
+
+def test_clip_from_two_threads(T):
+    import threading
+    sizes = [1 + (31 * i) % 900 for i in range(700)]
+    jobs, errors = [], []
+    for k in range(2):
+        _, grads = inputs(sizes[k:], 47 + k)
+        gs = grads()
+        params = [nn.Parameter(torch.zeros(len(g), device='cuda')) for g in gs]
+        norm = np.sqrt(sum(float(np.sum(g.astype(np.float64) ** 2)) for g in gs))
+        jobs.append((params, [f32(g) for g in gs], norm))
+
+    def work(params, gs, norm):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    for p, g in zip(params, gs):
+                        p.grad = g.clone()
+                    got = float(T.clip_grad_norm_(params, 1.0))
+                    assert abs(got - norm) <= 2 * U * norm, (got, norm)
+        except BaseException as e:   # noqa: B902 -- reported by the main thread
+            errors.append(e)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
 # ---- streams, graphs, re-pointed parameters ------------------------------------------------------------------------------
 @pytest.mark.parametrize('bits,count', [(32, 5), (8, 5), (32, 2500)])
 def test_captured_steps(T, bits, count):
@@ -680,3 +751,50 @@ def test_scheduler_drives_the_rate(T):
     assert opt.param_groups[0]['lr'] < 1e-2
     same(p, ref.p[0], 'p')
     assert float(opt.step(closure=lambda: torch.tensor(3.0))) == 3.0
+
+
+def _two_ranks(rank, port, q):
+    import os
+    import sys
+    sys.path[:0] = [os.path.dirname(os.path.dirname(os.path.abspath(__file__))), os.path.dirname(os.path.abspath(__file__))]
+    os.environ.update(MASTER_ADDR='127.0.0.1', MASTER_PORT=str(port))
+    import torch.distributed as dist
+    dist.init_process_group('gloo', rank=rank, world_size=2)
+    from super_resolution_amd import train
+    arrays, _ = inputs([700, 33], 131)
+    params = [nn.Parameter(f32(a) + rank) for a in arrays]      # replicas that start apart
+    opt = train.AdamW(params, state_bits=8, seed=4, **HP)
+    for p, g in zip(params, _rank_gradients(rank)):
+        p.grad = f32(g)
+    opt.step(clip_grad_norm=1.0)
+    torch.cuda.synchronize()
+    q.put((rank, [p.detach().cpu().tolist() for p in params], float(opt.grad_norm)))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def _rank_gradients(rank):
+    rng = np.random.default_rng(140 + rank)
+    return [rng.standard_normal(n).astype(np.float32) for n in (700, 33)]
+
+
+def test_two_ranks_average_their_gradients(T):
+    """Two processes on the one card, gradients exchanged over the host: both end with rank 0's parameters stepped by the mean."""
+    import os
+    import torch.multiprocessing as mp
+    ctx = mp.get_context('spawn')
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_two_ranks, args=(r, 35500 + os.getpid() % 2000, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    res = sorted(q.get(timeout=100) for _ in procs)
+    for p in procs:
+        p.join(60)
+        assert p.exitcode == 0
+    arrays, _ = inputs([700, 33], 131)
+    ref = R.Tensors(arrays, HP, 8, seed=4)
+    ref.step([(a + b) / np.float32(2) for a, b in zip(_rank_gradients(0), _rank_gradients(1))], 1.0)
+    for _, ps, norm in res:
+        for i, p in enumerate(ps):
+            same(torch.tensor(p), ref.p[i], 'p[%d]' % i)
+    assert res[0][2] == res[1][2]
