@@ -184,7 +184,8 @@ __global__ void image_from_planes_kernel(const TS* __restrict__ src, int H, int 
         const float r = clamp01(Elem<TS>::ld(p)), g = clamp01(Elem<TS>::ld(p + plane_stride)), b = clamp01(Elem<TS>::ld(p + 2 * plane_stride));
         TD* o = dst + i * dst_channels + dst_c0;
         if (gray) {
-            const float y = __fadd_rn(__fadd_rn(__fmul_rn(0.114f, b), __fmul_rn(0.587f, g)), __fmul_rn(0.299f, r));
+#pragma clang fp contract(off)  // (__fmul_rn and __fadd_rn are inlined as plain operators that may be fused)
+            const float y = (0.114f * b + 0.587f * g) + 0.299f * r;
             o[0] = (TD)rintf(__fmul_rn(y, full));
         } else {
             o[0] = (TD)rintf(__fmul_rn(b, full));
