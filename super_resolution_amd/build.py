@@ -9,8 +9,12 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 SOURCES = ['layout.hip', 'fbm.hip', 'fbm_fast.hip', 'fbm_fast_mixed.hip', 'fbm_mfma.hip', 'gates.hip', 'weightgen.hip', 'weightgen_bwd.hip', 'conv.hip', 'conv_plain.hip', 'net.hip', 'head.hip', 'train.hip', 'adamw.hip']
-# adamw.hip: every operation rounded once (its results are those of the formulas, bit for bit), and no packed float32 instructions
-EXTRA = {'adamw.hip': ['-ffp-contract=off', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']}
+# no packed float32 instructions: some of their forms have given wrong results on gfx950 now and then, and they gain nothing here
+# (batch of 16 512x512 images: 692.9 and 694.0 ms with them, 692.7 and 693.4 ms without)
+FLAGS = ['-O3', '--offload-arch=gfx950', '-std=c++17', '-fno-signed-zeros', '-fPIC', '-Wall', '-Wno-unused-result', '-Xclang', '-target-feature', '-Xclang',
+         '-packed-fp32-ops']
+# adamw.hip: every operation rounded once (its results are those of the formulas, bit for bit)
+EXTRA = {'adamw.hip': ['-ffp-contract=off']}
 OUT = os.path.join(HERE, 'libsr_amd.so')
 HOST_SRC = os.path.join(CSRC, 'torch_host.cpp')
 HOST_OUT = os.path.join(HERE, 'libsr_amd_torch.so')
@@ -62,8 +66,7 @@ def _build_kernels(force, verbose):
         src = os.path.join(CSRC, s)
         if not force and os.path.exists(o) and os.path.getmtime(o) > max(os.path.getmtime(src), newest_header):
             continue  # object is newer than its source and every header
-        cmd = [hipcc, '-O3', '--offload-arch=gfx950', '-std=c++17', '-fno-signed-zeros', '-fPIC', '-Wall', '-Wno-unused-result'] + EXTRA.get(s, []) + [
-               '-c', os.path.join(CSRC, s), '-o', o]
+        cmd = [hipcc] + FLAGS + EXTRA.get(s, []) + ['-c', os.path.join(CSRC, s), '-o', o]
         procs.append((cmd, subprocess.Popen(cmd)))
     for cmd, p in procs:
         if p.wait() != 0:

@@ -96,8 +96,8 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 __device__ __forceinline__ float lo_f(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float hi_f(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
-// g1*x + (g2-g1)*L2 + (g3-g2)*L4 + (1-g3)*L8 on 8 bf16 channels: channel pairs as float2, one v_pk_mul_f32 + three
-// v_pk_fma_f32 per pair (written as four products and three adds the compiler used ten instructions per pair)
+// g1*x + (g2-g1)*L2 + (g3-g2)*L4 + (1-g3)*L8 on 8 bf16 channels: channel pairs as float2, one product and
+// three fused multiply-adds per channel (written as four products and three adds the compiler used ten instructions per pair)
 typedef float float2v __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float2v unpack2(uint32_t u) {
     float2v r;

@@ -178,7 +178,7 @@ __device__ __forceinline__ void fft_pass_prime(const float2* __restrict__ src, f
         const int j = o / nu;
         const int jhi = j / Ns, k = j - jhi * Ns;
         const int ks = k * tstep;  // pass twiddle of operand t: tw[t * ks], t * ks < N
-        // complex numbers as float2v: sums / differences / scaled accumulations are one packed instruction each
+        // complex numbers as float2v: sums / differences / scaled accumulations in one expression each
         const float2v* srcv = (const float2v*)src;
         float2v a = srcv[j * P + p];
         if (premul) a *= premul[j];
