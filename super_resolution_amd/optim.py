@@ -47,6 +47,11 @@ def _on(dev):
     return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+def _stream(dev):
+    """The current stream of `dev` as the C ABI takes it (L.stream_ptr without the Python stream object: 2 us less a step)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
 class _Stage:
     """Host memory at `at` for a table of nbytes, and its way to the device.  Under capture it travels by value: a copy node would
     read the host buffer again at every replay."""
@@ -115,7 +120,6 @@ def _world(group):
 # ------------------------------------------------------------------------------------------------------------------
 # clipping
 # ------------------------------------------------------------------------------------------------------------------
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ (2-norm): scales the gradients in place by min(1, max_norm / (norm + 1e-6)) and returns the
     norm, a 0-d float32 tensor.  Squares are summed in float64, in an order that the shapes alone determine; nothing waits for
@@ -132,7 +136,7 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
         grads = [p.grad for p in params if p.grad is not None]
         dense = []
         for g in grads:
-            c = g if _is_dense(g) else g.contiguous()
+            c = g if _is_dense(g) else g.detach().contiguous()
             if c is not g:
                 odd.append(g)
             dense.append(c)
@@ -146,7 +150,7 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
         return torch.tensor(0.0)
     dev = torch.device('cuda', device.value)
     with _on(dev):
-        st = L.stream_ptr(dev)
+        st = _stream(dev)
         n32, n16 = counts[0], counts[1]
         stage = _Stage(16 * (n32 + n16))
         host.srt_take_spans(stage.at)
@@ -162,8 +166,9 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
         for l in lists:
             if l.nspans:
                 L.check(lib.sr_grad_scale(l.dtype, l.nspans, l.spans, l.on_host, buf.data_ptr() + 4 * buf.numel() - 4, st), 'sr_grad_scale')
-        for g in odd:
-            g.mul_(buf[-1])
+        with torch.no_grad() if odd else contextlib.nullcontext():
+            for g in odd:
+                g.mul_(buf[-1])
     return norm
 
 
@@ -203,7 +208,8 @@ class _List:
         self.dtype = self.params[0].dtype
         self.handle, self.tracked, self.retired = None, None, []
         self.steps = 0              # int: all tensors alike; else an int64 array
-        self.ptrs = self.stage = None
+        # by-value tables are read by the launch itself: one buffer serves every step
+        self.ptrs, self.stage = None, _Stage(8 * self.n) if self.n <= L.ADAMW_BY_VALUE else None
         self.odd = (C.c_int64 * self.n)()
         self.nodd, self.moved = C.c_int64(), C.c_int64()
         self.seen = self.step_dev = self.scalars = None
@@ -251,8 +257,10 @@ class _List:
 
     def gradients(self, keep):
         """Fills self.ptrs; returns the number of tensors without a gradient.  keep: copies that must live until the launch."""
-        self.stage = stage = _Stage(8 * self.n)
-        self.ptrs = (C.c_uint64 * self.n).from_address(stage.at)
+        if self.n > L.ADAMW_BY_VALUE or self.ptrs is None:
+            if self.n > L.ADAMW_BY_VALUE:
+                self.stage = _Stage(8 * self.n)
+            self.ptrs = (C.c_uint64 * self.n).from_address(self.stage.at)
         missing = _host_lib().srt_gradients(self.tracked, self.ptrs, self.odd, C.byref(self.nodd), C.byref(self.moved))
         if missing < 0:
             _host_failed('AdamW')
@@ -433,7 +441,7 @@ class AdamW(torch.optim.Optimizer):
             m, v = (torch.empty(self.numel, dtype=dtype, device=self.device) for _ in range(2))
             for lst in self._lists:
                 if self.numel:
-                    L.check(L.lib().sr_adamw_moments(lst.handle, code, m.data_ptr(), v.data_ptr(), L.stream_ptr(self.device)), 'sr_adamw_moments')
+                    L.check(L.lib().sr_adamw_moments(lst.handle, code, m.data_ptr(), v.data_ptr(), _stream(self.device)), 'sr_adamw_moments')
         return m, v
 
     def ema_parameters(self):
@@ -455,7 +463,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError('AdamW: clip_grad_norm must not be negative (got %r)' % (clip_grad_norm,))
         dev = self.device
         with _on(dev):
-            st = L.stream_ptr(dev)
+            st = _stream(dev)
             capturing = torch.cuda.is_current_stream_capturing()
             if capturing and not self.capturable:
                 raise RuntimeError('AdamW: a step under graph capture needs capturable=True (the step count would stay what it is now)')
@@ -605,7 +613,7 @@ class AdamW(torch.optim.Optimizer):
             if self.numel:
                 m, v = flat('exp_avg'), flat('exp_avg_sq')
                 for lst in self._lists:
-                    L.check(L.lib().sr_adamw_set_moments(lst.handle, m.data_ptr(), v.data_ptr(), self.seed, L.stream_ptr(self.device)),
+                    L.check(L.lib().sr_adamw_set_moments(lst.handle, m.data_ptr(), v.data_ptr(), self.seed, _stream(self.device)),
                             'sr_adamw_set_moments')
             for lst, t in zip(self._lists, steps):
                 if self.capturable:
