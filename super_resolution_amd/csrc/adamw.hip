@@ -19,10 +19,16 @@
 // was decoded encodes to itself, so a checkpoint in float32 resumes where it was.  A block with a NaN or an infinity has the
 // exponent byte 255 and decodes to NaN as a whole.
 //
-// What bounds it: memory.  Every value is read and written once (28 bytes of float32 state, 16 with 8-bit moments) against 40 to
-// 90 vector instructions.  Work is split into pieces of 1024 consecutive values of one tensor, one per WAVE: RRDBNet-FDConv has
-// 8380 tensors of which 8000 are smaller than a piece, and a workgroup each would leave three of its four waves idle.  A wave
-// issues the loads of its four groups of 256 values (16 bytes per lane and tensor) before it computes.
+// What bounds it: memory.  Every value is read and written once: 28 bytes with float32 moments, 16 with 8-bit ones.  256 M float32
+// values take 1.39 ms, 5.15 TB/s; four arrays read and three written at once is what costs against the 5.9 TB/s of one array scaled
+// in place (5.65 for three read and one written): with the arithmetic taken out the time is the same.  8-bit moments: 128 M float32
+// values 0.39 ms, 5.2 TB/s; with bfloat16 weights (10 bytes, 76 vector instructions a value) 96 M take 0.19 to 0.25 ms, and their
+// instructions alone 0.19 to issue.
+// Work is split into pieces of 1024 consecutive values of one tensor, one per WAVE: most of RRDBNet-FDConv's 8380 tensors are
+// smaller than a piece, and a workgroup each would leave three of its four waves idle.  A wave issues the loads of its four groups
+// of 256 values (16 bytes per lane and tensor) before it computes, and stores group by group.  Measured against that, on 256 M
+// values: pieces of 512 +4 %, of 2048 +1 % (8 bits: +6 %, with bfloat16 +40 %), all loads of one array together +4 %, all stores
+// at the end +5 %, nontemporal loads +7 %, stores +1 %, a contiguous eighth per XCD -2 % but +5 to 8 % with 8 bits or bfloat16.
 #include "common.h"
 
 #include <math.h>
@@ -53,7 +59,7 @@ struct Piece {
 };
 
 // The gradients' addresses: they are new tensors every step, and a kernel cannot follow a host list.  Short lists travel in the
-// kernel's arguments (no copy, no second launch: 28 -> 21 us for a step of 53 tensors), long ones lie on the device.
+// kernel's arguments (no copy, no second launch: 8 us of a step of 53 tensors), long ones lie on the device.
 struct GradsAt {
     const void* const* at;
     __device__ __forceinline__ const void* operator[](uint32_t i) const { return at[i]; }
@@ -534,8 +540,12 @@ __global__ __launch_bounds__(256) void adamw_set_moments_kernel(const Rec* __res
 }
 
 // ---- global gradient norm ---------------------------------------------------------------------------------------------
-// Squares are added in float64 (a float32 square overflows from 1.8e19 on, and 1e8 of them lose three digits), in an order
-// that the shapes alone determine.  Work items are runs of consecutive values; waves take them in turn.
+// Squares are added in float64 (a float32 square overflows from 1.8e19 on, and 1e8 of them lose three digits; float64 multiply-adds
+// run at the float32 rate here), in an order that the shapes alone determine.  Work items are runs of consecutive values; waves
+// take them in turn, four 16-byte loads of every lane in flight (256 M bfloat16 values: norm 0.10 ms, 5 TB/s; scaling 0.18 ms, 5.6
+// TB/s, 0.21 with one 8-byte load at a time).  Right after a step the norm of 48 M bfloat16 values takes 37 us instead of 25: the
+// memory-side cache is full of what the step wrote, and every line read pushes one out.  Two or four pieces at a time did not
+// change that.
 template <typename G>
 struct PieceSource {  // the pieces of an optimizer's list, gradients by tensor
     const Rec* recs;
