@@ -271,7 +271,7 @@ __device__ __forceinline__ uint16_t round_bf16(float x, uint32_t h) {
 // instructions, which is what bounds the step with 8-bit moments.  rsq / rcp are good to one ulp; one correction by the exact
 // residual rounds the root correctly (checked for all 2^24 significands) and the reciprocal (all 2^23), and with a correctly
 // rounded reciprocal the same correction rounds the quotient correctly (Markstein's theorem).  The ranges below keep every
-// residual exact: 0 <= x < 2^124, no subnormals but 0; |a| 0 or in [2^-85, 2^84], b in [2^-40, 2^31].
+// residual exact: 0 <= x < 2^124, no subnormals but 0; |a| 0 or in [2^-85, 2^84], b in [2^-40, 2^41].
 __device__ __forceinline__ float root(float x) {
     const float y = __builtin_amdgcn_rsqf(fmaxf(x, 0x1p-100f));
     const float r = x * y;

@@ -115,7 +115,7 @@ SRT_API int64_t srt_gradients(void* h, uint64_t* out, int64_t* odd, int64_t* nod
             const c10::TensorImpl* g = grad->unsafeGetTensorImpl();
             // (equal key sets: the same kind of tensor on the same kind of device)
             if (g->key_set() == p->key_set() && g->numel() == was.numel && g->dtype() == was.dtype && g->device() == was.device && same_layout(g, p))
-                out[i] = (uint64_t)(uintptr_t)g->data();
+                out[i] = g->numel() ? (uint64_t)(uintptr_t)g->data() : 16;  // (of an empty tensor nothing is read, but it has one)
             else
                 odd[(*nodd)++] = (int64_t)i;
         }

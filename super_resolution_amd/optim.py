@@ -200,8 +200,10 @@ def _norm(lists, max_norm, dev, st):
 class _List:
     """The tensors of one parameter group with one dtype: the device tables, and the walk over their gradients."""
 
+    buried = []   # handles dropped while a stream was capturing, where freeing is not allowed
+
     def __init__(self, opt, group, bits, members):
-        self.group, self.bits, self.members = group, bits, members   # members: indices into opt.params
+        self.group, self.bits, self.members = group, bits, members   # indices into opt.param_groups and opt.params
         self.params = [opt.params[i] for i in members]
         self.n = len(members)
         self.sizes = [p.numel() for p in self.params]
@@ -234,6 +236,8 @@ class _List:
         if not tracked:
             L.lib().sr_adamw_destroy(h)
             _host_failed('AdamW')
+        while self.buried and not torch.cuda.is_current_stream_capturing():
+            L.lib().sr_adamw_destroy(self.buried.pop())
         old = (self.handle, self.tracked)
         self.handle, self.tracked = h, tracked
         if opt.capturable and old[0]:
@@ -241,10 +245,13 @@ class _List:
         else:
             self._free(*old)
 
-    @staticmethod
-    def _free(handle, tracked):
+    @classmethod
+    def _free(cls, handle, tracked):
         if handle:
-            L.lib().sr_adamw_destroy(handle)
+            if torch.cuda.is_current_stream_capturing():
+                cls.buried.append(handle)
+            else:
+                L.lib().sr_adamw_destroy(handle)
         if tracked:
             _host_lib().srt_untrack(tracked)
 
@@ -360,11 +367,11 @@ class AdamW(torch.optim.Optimizer):
                 self.ema = torch.empty(total, dtype=torch.float32, device=dev)
                 self._reset_ema()
             self._lists, first = [], 0
-            for g in self.param_groups:
+            for k, g in enumerate(self.param_groups):
                 for dt in (torch.float32, torch.bfloat16):
                     members = [first + i for i, p in enumerate(g['params']) if p.dtype == dt]
                     if members:
-                        self._lists.append(_List(self, g, g['state_bits'], members))
+                        self._lists.append(_List(self, k, g['state_bits'], members))
                 first += len(g['params'])
             if len(self._lists) > L.GRAD_MAX_LISTS:
                 raise ValueError('AdamW: at most %d parameter groups of one dtype' % L.GRAD_MAX_LISTS)
@@ -469,7 +476,7 @@ class AdamW(torch.optim.Optimizer):
                 raise RuntimeError('AdamW: a step under graph capture needs capturable=True (the step count would stay what it is now)')
             keep, hypers, missing = [], [], []
             for lst in self._lists:   # everything that can fail comes before the first launch
-                hypers.append(self._hyper(lst.group))
+                hypers.append(self._hyper(self.param_groups[lst.group]))
                 missing.append(lst.gradients(keep))
                 if lst.moved.value:
                     self._follow(lst, capturing)
@@ -497,7 +504,7 @@ class AdamW(torch.optim.Optimizer):
                 run(1, None, table)
             return
         if self.capturable:
-            lr = lst.group['lr']
+            lr = self.param_groups[lst.group]['lr']
             L.check(lib.sr_adamw_tick(C.byref(h), lr.data_ptr() if torch.is_tensor(lr) and lr.is_cuda else None, lst.step_dev.data_ptr(),
                                       lst.scalars.data_ptr(), st), 'sr_adamw_tick')
             run(0, lst.scalars.data_ptr(), table)
@@ -560,11 +567,10 @@ class AdamW(torch.optim.Optimizer):
         if any(steps.values()):
             m, v = self.moments()
             ema = self.ema.clone() if self.ema is not None else None
-            for i in range(len(self.params)):
-                if steps[i]:
-                    state[i] = {'step': torch.tensor(float(steps[i])), 'exp_avg': self._shaped(m, i), 'exp_avg_sq': self._shaped(v, i)}
-                if ema is not None:
-                    state.setdefault(i, {})['ema'] = self._shaped(ema, i)
+            for i in (i for i in range(len(self.params)) if steps[i]):
+                state[i] = {'step': torch.tensor(float(steps[i])), 'exp_avg': self._shaped(m, i), 'exp_avg_sq': self._shaped(v, i)}
+                if ema is not None:     # (the average of a parameter that never moved is the parameter)
+                    state[i]['ema'] = self._shaped(ema, i)
         groups, first = [], 0
         for g in self.param_groups:
             hp = {k: x for k, x in g.items() if k != 'params'}
@@ -584,6 +590,8 @@ class AdamW(torch.optim.Optimizer):
         place = {}
         for i, key in enumerate(k for g in groups for k in g['params']):
             place[key] = i
+        if any(k not in place for k in sd['state']):
+            raise ValueError('AdamW.load_state_dict: a state for a parameter that no group holds')
         state = {place[k]: s for k, s in sd['state'].items()}
         for i, s in state.items():
             for name in ('exp_avg', 'exp_avg_sq', 'ema'):

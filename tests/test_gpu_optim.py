@@ -171,6 +171,29 @@ def test_missing_gradients_keep_their_own_count(T, bits):
             assert np.abs(p.detach().cpu().numpy() - q.detach().numpy()).max() <= 6 * 16 * U * 5
 
 
+def test_empty_parameters_count_their_steps(T):
+    p = [nn.Parameter(torch.ones(5, device='cuda')), nn.Parameter(torch.zeros(0, device='cuda')), nn.Parameter(torch.ones(700, device='cuda'))]
+    opt = T.AdamW(p, ema_decay=0.9)
+    for have in ((1, 1, 1), (0, 1, 1), (1, 1, 1), (0, 0, 0), (1, 1, 0)):
+        for q, h in zip(p, have):
+            q.grad = torch.ones_like(q) if h else None
+        opt.step()
+    sd = opt.state_dict()
+    assert [int(sd['state'][i]['step']) for i in range(3)] == [3, 4, 3]
+    never = T.AdamW([nn.Parameter(torch.ones(5, device='cuda')), nn.Parameter(torch.ones(5, device='cuda'))], ema_decay=0.9)
+    never.params[0].grad = torch.ones(5, device='cuda')
+    never.step()
+    assert sorted(never.state_dict()['state']) == [0]       # as torch: a parameter without a step has no state
+    twin = [nn.Parameter(q.detach().clone()) for q in never.params]
+    topt = torch.optim.AdamW(twin)
+    topt.load_state_dict(never.state_dict())
+    for q in twin:
+        q.grad = torch.ones(5, device='cuda')
+    topt.step()
+    with pytest.raises(ValueError, match='no group'):
+        never.load_state_dict({'state': {7: {}}, 'param_groups': never.state_dict()['param_groups']})
+
+
 def test_layouts(T):
     """Parameters in channels_last memory, gradients in another order, expanded, or with holes."""
     torch.manual_seed(1)
@@ -724,7 +747,7 @@ def test_train_step_with_adamw(T, bits):
     for (n, p), q, s, e in zip(net.named_parameters(), twin.parameters(), start, opt.ema_parameters()):
         # one step is at most lr; m and v are not rounded before it: float32 roundings of p and of the update (the clip factors
         # differ by FlatAdam's float32 norm of 20000 terms, 2^-13 of the gradient, which eps alone turns into a difference)
-        assert float((p - q).abs().max()) <= 4 * U * float(s.abs().max()) + 1e-3 * 2 ** -12, n
+        assert float((p - q).detach().abs().max()) <= 4 * U * float(s.abs().max()) + 1e-3 * 2 ** -12, n
         assert torch.allclose(e, 0.5 * s + 0.5 * p.detach(), rtol=4 * U, atol=4 * U * float(s.abs().max())), n
     # evaluation after the step sees the new weights (FDConv keys its cached bases on the version counters)
     net.eval()
