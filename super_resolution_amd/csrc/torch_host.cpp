@@ -42,7 +42,7 @@ struct Tracked {
         const void* data;
         int64_t numel;
         caffe2::TypeMeta dtype;
-        c10::Device device;
+        bool counts;  // has a version counter
     };
     std::vector<Was> was;
 };
@@ -78,7 +78,7 @@ SRT_API void* srt_track(PyObject* list) {
             const at::Tensor& p = tensor_of(PyList_GET_ITEM(list, i));
             t->params.push_back(p);
             const c10::TensorImpl* impl = p.unsafeGetTensorImpl();
-            t->was.push_back({impl->data(), impl->numel(), impl->dtype(), impl->device()});
+            t->was.push_back({impl->data(), impl->numel(), impl->dtype(), !p.is_inference()});
         }
         return 0;
     });
@@ -104,17 +104,17 @@ SRT_API int64_t srt_gradients(void* h, uint64_t* out, int64_t* odd, int64_t* nod
         for (size_t i = 0; i < n; ++i) {
             c10::TensorImpl* p = t.params[i].unsafeGetTensorImpl();
             const Tracked::Was& was = t.was[i];
-            if (p->data() != was.data || p->numel() != was.numel || p->dtype() != was.dtype || p->device() != was.device) ++*moved;
+            if (p->data() != was.data || p->numel() != was.numel || p->dtype() != was.dtype) ++*moved;  // (another device: other data)
             const at::Tensor* grad = gradient_of(p);
             out[i] = 0;
             if (!grad) {
                 ++missing;
                 continue;
             }
-            if (!p->is_inference()) p->bump_version();
+            if (was.counts) p->bump_version();
             const c10::TensorImpl* g = grad->unsafeGetTensorImpl();
-            // (equal key sets: the same kind of tensor on the same kind of device)
-            if (g->key_set() == p->key_set() && g->numel() == was.numel && g->dtype() == was.dtype && g->device() == was.device && same_layout(g, p))
+            // (equal key sets: the same kind of tensor; torch keeps a gradient on its parameter's device)
+            if (g->key_set() == p->key_set() && g->numel() == was.numel && g->dtype() == was.dtype && same_layout(g, p))
                 out[i] = g->numel() ? (uint64_t)(uintptr_t)g->data() : 16;  // (of an empty tensor nothing is read, but it has one)
             else
                 odd[(*nodd)++] = (int64_t)i;

@@ -220,18 +220,19 @@ class _List:
             self.scalars = torch.empty(L.ADAMW_SCALARS_BYTES, dtype=torch.uint8, device=opt.device)
 
     def build(self, opt):
-        arr = (L.AdamWTensor * self.n)()
-        for t, i, p in zip(arr, self.members, self.params):
-            t.p, t.n, t.index = p.data_ptr(), p.numel(), opt._index[i]
-            if self.bits == 32:
-                t.m = opt._m32.data_ptr() + 4 * opt._at[i]
-                t.v = opt._v32.data_ptr() + 4 * opt._at[i]
-            else:
-                t.m, t.v = opt._m8.data_ptr() + opt._at[i], opt._v8.data_ptr() + opt._at[i]
-                t.me, t.ve = opt._me.data_ptr() + opt._block[i], opt._ve.data_ptr() + opt._block[i]
-            t.ema = opt.ema.data_ptr() + 4 * opt._index[i] if opt.ema is not None else None
+        t = np.zeros(self.n, dtype=np.dtype([(name, np.int64) for name, _ in L.AdamWTensor._fields_]))
+        index, at, block = (x[self.members] for x in (opt._index, opt._at, opt._block))
+        t['p'], t['n'], t['index'] = [p.data_ptr() for p in self.params], self.sizes, index
+        if self.bits == 32:
+            t['m'], t['v'] = opt._m32.data_ptr() + 4 * at, opt._v32.data_ptr() + 4 * at
+        else:
+            t['m'], t['v'] = opt._m8.data_ptr() + at, opt._v8.data_ptr() + at
+            t['me'], t['ve'] = opt._me.data_ptr() + block, opt._ve.data_ptr() + block
+        if opt.ema is not None:
+            t['ema'] = opt.ema.data_ptr() + 4 * index
         h = C.c_void_p()
-        L.check(L.lib().sr_adamw_create(L.dtype_code(self.dtype), self.bits, self.n, arr, C.byref(h)), 'sr_adamw_create')
+        L.check(L.lib().sr_adamw_create(L.dtype_code(self.dtype), self.bits, self.n, t.ctypes.data_as(C.POINTER(L.AdamWTensor)), C.byref(h)),
+                'sr_adamw_create')
         tracked = _host_lib().srt_track(self.params)
         if not tracked:
             L.lib().sr_adamw_destroy(h)
@@ -344,18 +345,15 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError('AdamW: a parameter with holes or repeated elements')
         self._check_overlap()
         # places: element number among all parameters; offset among the tensors of the same kind of moments; first block
-        self._index, self._at, self._block, total, n = [], [], [], 0, {32: 0, 8: 0}
-        blocks = 0
-        for g in self.param_groups:
-            for p in g['params']:
-                k = p.numel()
-                self._index.append(total)
-                self._at.append(n[g['state_bits']])
-                self._block.append(blocks)
-                total += k
-                n[g['state_bits']] += k
-                blocks += -(-k // L.ADAMW_BLOCK) if g['state_bits'] == 8 else 0
-        self.numel = total
+        size = np.array([p.numel() for p in self.params], dtype=np.int64)
+        bits = np.repeat([g['state_bits'] for g in self.param_groups], [len(g['params']) for g in self.param_groups])
+        in_8 = np.where(bits == 8, size, 0)
+        in_32, in_blocks = size - in_8, -(-in_8 // L.ADAMW_BLOCK)
+        before = lambda x: np.cumsum(x) - x     # noqa: E731
+        self._index, self._block = before(size), before(in_blocks)
+        self._at = np.where(bits == 8, before(in_8), before(in_32))
+        n, blocks = {32: int(in_32.sum()), 8: int(in_8.sum())}, int(in_blocks.sum())
+        self.numel = total = int(size.sum())
         with torch.cuda.device(dev), torch.no_grad():
             if broadcast and _world(group) > 1:
                 _broadcast_parameters(self.params, group)
@@ -424,8 +422,8 @@ class AdamW(torch.optim.Optimizer):
 
     def _shaped(self, flat, i):
         """Tensor i's part of a flat array, in the parameter's shape and strides."""
-        p = self.params[i]
-        return flat[self._index[i]:self._index[i] + p.numel()].as_strided(p.shape, p.stride())
+        p, at = self.params[i], int(self._index[i])
+        return flat[at:at + p.numel()].as_strided(p.shape, p.stride())
 
     @property
     def exp_avg(self):
@@ -539,8 +537,9 @@ class AdamW(torch.optim.Optimizer):
         lst.build(self)
 
     def _check_overlap(self):
-        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
-        if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        spans = np.array([(p.data_ptr(), p.numel() * p.element_size()) for p in self.params if p.numel()], dtype=np.int64).reshape(-1, 2)
+        spans = spans[np.argsort(spans[:, 0])]
+        if (spans[1:, 0] < spans[:-1].sum(1)).any():
             raise ValueError('AdamW: two parameters share memory')
 
     def _same_gradients(self, lst):
@@ -595,7 +594,7 @@ class AdamW(torch.optim.Optimizer):
         state = {place[k]: s for k, s in sd['state'].items()}
         for i, s in state.items():
             for name in ('exp_avg', 'exp_avg_sq', 'ema'):
-                if name in s and tuple(s[name].shape) != tuple(self.params[i].shape):
+                if name in s and s[name].shape != self.params[i].shape:
                     raise ValueError('AdamW.load_state_dict: parameter %d has shape %s, its %s %s'
                                      % (i, tuple(self.params[i].shape), name, tuple(s[name].shape)))
         new = [{k: g.get(k, mine[k]) for k in ('lr', 'betas', 'eps', 'weight_decay')} for g, mine in zip(groups, self.param_groups)]
