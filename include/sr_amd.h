@@ -419,6 +419,11 @@ int sr_grad_scale(int dtype, int64_t nspans, const sr_grad_span* spans, int on_h
 /* Copies a small HOST array (tables of pointers) to the device through kernel arguments: by value, so the source may be reused at
  * once and a captured graph keeps what it held; 3840 bytes per launch.  bytes and dst: multiples of 4. */
 int sr_upload(const void* src_host, void* dst, size_t bytes, void* stream);
+/* The same for larger tables, from PINNED host memory that a kernel reads where it lies (a copy-engine transfer of 67 KB and its
+ * hand-over to the next kernel take 27 us, this 4; src and dst 16-byte aligned).  The kernel then writes `ticket` to SR_UPLOAD_WORDS words at `done`,
+ * pinned host memory too: when all of them hold it the source may be written again. */
+#define SR_UPLOAD_WORDS 8
+int sr_upload_pinned(const void* src_pinned, void* dst, size_t bytes, int64_t* done, int64_t ticket, void* stream);
 
 /* ---- whole network (RRDBNet.forward) ------------------------------------------------------- */
 typedef struct sr_rrdbnet sr_rrdbnet;

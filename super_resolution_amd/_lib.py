@@ -69,7 +69,7 @@ class GradList(C.Structure):
                 ('on_host', C.c_int32)]
 
 
-ADAMW_BLOCK, ADAMW_SCALARS_BYTES, ADAMW_SKIP, ADAMW_BY_VALUE, GRAD_MAX_LISTS, GRAD_SPANS_BY_VALUE = 256, 64, 1, 448, 64, 224
+ADAMW_BLOCK, ADAMW_SCALARS_BYTES, ADAMW_SKIP, ADAMW_BY_VALUE, GRAD_MAX_LISTS, GRAD_SPANS_BY_VALUE, UPLOAD_WORDS = 256, 64, 1, 448, 64, 224, 8
 
 _SIGS = {
     'sr_strerror': (C.c_char_p, [C.c_int]),
@@ -152,6 +152,7 @@ _SIGS = {
     'sr_grad_norm': (C.c_int, [C.c_int, C.POINTER(GradList), C.c_double, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     'sr_grad_scale': (C.c_int, [C.c_int, C.c_int64, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p]),
     'sr_upload': (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    'sr_upload_pinned': (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_int64, C.c_void_p]),
     'sr_debug_force_generic_conv': (None, [C.c_int]),
     'sr_debug_force_generic_fft': (None, [C.c_int]),
     'sr_debug_no_mixed_fft': (None, [C.c_int]),

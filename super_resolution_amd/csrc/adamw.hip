@@ -716,6 +716,18 @@ __global__ __launch_bounds__(256) void upload_kernel(UploadArgs a) {
     for (int i = threadIdx.x; i < a.bytes / 4; i += 256) ((uint32_t*)a.dst)[i] = a.data[i];
 }
 
+// A word per workgroup, written behind its barrier, tells that it has read its part: no counter that would have to be cleared.
+// 128 KB of reads across the host link in flight (one workgroup alone: 67 KB in 9 us instead of 4).
+constexpr uint32_t PINNED_WG = 1024, PINNED_ALL = PINNED_WG * SR_UPLOAD_WORDS;
+__global__ __launch_bounds__(PINNED_WG) void upload_pinned_kernel(const uint32_t* __restrict__ src, uint32_t* __restrict__ dst, uint32_t words,
+                                                                  int64_t* done, int64_t ticket) {
+    const uint32_t quads = words / 4, me = blockIdx.x * PINNED_WG + threadIdx.x;
+    for (uint32_t i = me; i < quads; i += PINNED_ALL) ((uint4*)dst)[i] = ((const uint4*)src)[i];
+    if (me < (words & 3)) dst[quads * 4 + me] = src[quads * 4 + me];
+    __syncthreads();
+    if (threadIdx.x == 0) __hip_atomic_store(done + blockIdx.x, ticket, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+
 }  // namespace sr
 
 using namespace sr;
@@ -984,5 +996,13 @@ extern "C" int sr_upload(const void* src_host, void* dst, size_t bytes, void* st
         upload_kernel<<<1, 256, 0, (hipStream_t)stream>>>(a);
         SR_LAUNCH_CHECK();
     }
+    return SR_OK;
+}
+
+extern "C" int sr_upload_pinned(const void* src_pinned, void* dst, size_t bytes, int64_t* done, int64_t ticket, void* stream) {
+    SR_REQUIRE(bytes % 4 == 0 && bytes > 0 && bytes <= ((size_t)1 << 30) && src_pinned && dst && done);
+    SR_REQUIRE((uintptr_t)dst % 16 == 0 && (uintptr_t)src_pinned % 16 == 0 && (uintptr_t)done % 8 == 0);
+    upload_pinned_kernel<<<SR_UPLOAD_WORDS, PINNED_WG, 0, (hipStream_t)stream>>>((const uint32_t*)src_pinned, (uint32_t*)dst, (uint32_t)(bytes / 4), done, ticket);
+    SR_LAUNCH_CHECK();
     return SR_OK;
 }

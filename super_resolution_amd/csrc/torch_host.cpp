@@ -140,6 +140,7 @@ SRT_API int64_t srt_spans(PyObject* list, int of_params, int* device, int64_t* c
         bool ascending = true;
         const Py_ssize_t size = PyList_GET_SIZE(list);
         found[0].reserve(size);
+        c10::DispatchKeySet usual;  // of the first gradient: those with the same keys are of the same kind
         for (Py_ssize_t i = 0; i < size; ++i) {
             c10::TensorImpl* g = tensor_of(PyList_GET_ITEM(list, i)).unsafeGetTensorImpl();
             if (of_params) {
@@ -148,9 +149,12 @@ SRT_API int64_t srt_spans(PyObject* list, int of_params, int* device, int64_t* c
                 g = grad->unsafeGetTensorImpl();
             }
             ++counts[2];
-            if (!g->is_inference()) g->bump_version();  // they are about to be written
-            if (g->layout() != at::kStrided || !g->device().is_cuda()) return 1 + i;
-            if (*device < 0) *device = g->device().index();
+            if (!(g->key_set() == usual)) {
+                if (g->layout() != at::kStrided || !g->device().is_cuda()) return 1 + i;
+                if (*device < 0) *device = g->device().index();
+                if (!g->is_inference()) usual = g->key_set();
+            }
+            if (g->key_set() == usual) g->bump_version();  // they are about to be written
             const int kind = g->dtype() == caffe2::TypeMeta::Make<float>() ? 0 : g->dtype() == caffe2::TypeMeta::Make<at::BFloat16>() ? 1 : -1;
             if (kind < 0 || g->device().index() != *device) return 1 + i;
             if (!g->is_contiguous() && !g->is_non_overlapping_and_dense()) return -2 - i;

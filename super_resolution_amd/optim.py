@@ -10,6 +10,7 @@ one kernel (csrc/adamw.hip) walks all tensors of a group, reads gradients, param
 import contextlib
 import ctypes as C
 import os
+import threading
 
 import numpy as np
 import torch
@@ -18,7 +19,7 @@ from . import _lib as L
 
 _HOST_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), 'libsr_amd_torch.so')
 _host = None
-_BY_VALUE = 3840   # bytes of a table that go to the device as kernel arguments, in one launch; longer ones are copied
+_BY_VALUE = 3840   # bytes of a table that go to the device as kernel arguments, in one launch; longer ones are read from pinned memory
 
 
 def _host_lib():
@@ -52,9 +53,39 @@ def _stream(dev):
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
+class _Pinned:
+    """A block of pinned memory: words that the GPU writes when it has read the rest, and the table behind them."""
+
+    free = []                   # blocks that were handed to a kernel; ready() tells whether it has read them
+    lock = threading.Lock()
+
+    def __init__(self, nbytes):
+        self.size = 1 << max(13, (nbytes - 1).bit_length())
+        self.memory = torch.zeros(8 * L.UPLOAD_WORDS + self.size, dtype=torch.uint8, pin_memory=True)
+        self.done = self.memory.data_ptr()
+        self.table = self.done + 8 * L.UPLOAD_WORDS
+        self.ticket, self.expected = 0, bytes(8 * L.UPLOAD_WORDS)
+
+    def next_ticket(self):
+        self.ticket += 1
+        self.expected = self.ticket.to_bytes(8, 'little') * L.UPLOAD_WORDS
+        return self.ticket
+
+    def ready(self):
+        return C.string_at(self.done, 8 * L.UPLOAD_WORDS) == self.expected
+
+    @classmethod
+    def take(cls, nbytes):
+        with cls.lock:
+            for i, b in enumerate(cls.free):
+                if b.size >= nbytes and b.ready():
+                    return cls.free.pop(i)
+        return cls(nbytes)
+
+
 class _Stage:
-    """Host memory at `at` for a table of nbytes, and its way to the device.  Under capture it travels by value: a copy node would
-    read the host buffer again at every replay."""
+    """Host memory at `at` for a table of nbytes, and its way to the device.  Under capture it travels by value: what a captured kernel
+    or copy reads from the host is read again at every replay."""
 
     def __init__(self, nbytes):
         self.nbytes = nbytes
@@ -63,15 +94,18 @@ class _Stage:
             self.host = (C.c_char * max(nbytes, 1))()
             self.at = C.addressof(self.host)
         else:
-            self.host = torch.empty(nbytes, dtype=torch.uint8, pin_memory=True)
-            self.at = self.host.data_ptr()
+            self.host = _Pinned.take(nbytes)
+            self.at = self.host.table
 
     def upload(self, dev, st):
         table = torch.empty(max(self.nbytes, 1), dtype=torch.uint8, device=dev)
         if self.by_value:
             L.check(L.lib().sr_upload(self.at, table.data_ptr(), self.nbytes, st), 'sr_upload')
         else:
-            table.copy_(self.host, non_blocking=True)   # torch keeps the pinned block until the copy is done
+            block = self.host
+            L.check(L.lib().sr_upload_pinned(self.at, table.data_ptr(), self.nbytes, block.done, block.next_ticket(), st), 'sr_upload_pinned')
+            with _Pinned.lock:
+                _Pinned.free.append(block)
         return table
 
 
@@ -282,6 +316,8 @@ class _List:
                 g = torch.empty_like(p).copy_(g)
             keep.append(g)
             self.ptrs[self.odd[k]] = g.data_ptr()
+        # kept for what looks at them after the table has gone: its memory is given back with the upload
+        self.copy = np.frombuffer(self.ptrs, dtype=np.uint64).copy() if missing or not isinstance(self.steps, int) else None
         return missing
 
     def table(self, dev, st, ptrs=None):
@@ -513,7 +549,7 @@ class AdamW(torch.optim.Optimizer):
             return
         # step counts differ: one launch per count, the other tensors marked; the first one also takes those without a gradient
         # (their averages)
-        ptrs = np.frombuffer(lst.ptrs, dtype=np.uint64)
+        ptrs = lst.copy
         have = ptrs != 0
         steps = np.full(lst.n, lst.steps, dtype=np.int64) if isinstance(lst.steps, int) else lst.steps
         lst.steps = steps = steps + have

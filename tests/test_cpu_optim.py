@@ -33,13 +33,13 @@ def host(L):
 
 def test_structs_match_the_header(L):
     src = '#include <stdio.h>\n#include "sr_amd.h"\nint main(){printf("%zu %zu %zu %zu %d %d %d\\n", sizeof(sr_adamw_tensor), ' \
-          'sizeof(sr_adamw_hyper), sizeof(sr_grad_list), sizeof(sr_grad_span), SR_ADAMW_BLOCK, SR_ADAMW_SCALARS_BYTES, SR_GRAD_MAX_LISTS);printf("%d %d\\n", SR_ADAMW_BY_VALUE, SR_GRAD_SPANS_BY_VALUE);return 0;}\n'
+          'sizeof(sr_adamw_hyper), sizeof(sr_grad_list), sizeof(sr_grad_span), SR_ADAMW_BLOCK, SR_ADAMW_SCALARS_BYTES, SR_GRAD_MAX_LISTS);printf("%d %d %d\\n", SR_ADAMW_BY_VALUE, SR_GRAD_SPANS_BY_VALUE, SR_UPLOAD_WORDS);return 0;}\n'
     with tempfile.TemporaryDirectory() as d:
         open(os.path.join(d, 'a.c'), 'w').write(src)
         subprocess.check_call(['gcc', '-I', os.path.join(ROOT, 'include'), os.path.join(d, 'a.c'), '-o', os.path.join(d, 'a')])
         got = [int(x) for x in subprocess.check_output([os.path.join(d, 'a')]).split()]
     assert got == [C.sizeof(L.AdamWTensor), C.sizeof(L.AdamWHyper), C.sizeof(L.GradList), 16, L.ADAMW_BLOCK, L.ADAMW_SCALARS_BYTES, L.GRAD_MAX_LISTS,
-                   L.ADAMW_BY_VALUE, L.GRAD_SPANS_BY_VALUE]
+                   L.ADAMW_BY_VALUE, L.GRAD_SPANS_BY_VALUE, L.UPLOAD_WORDS]
 
 
 def test_c_entries_refuse_bad_arguments(L):
@@ -92,6 +92,9 @@ def test_c_entries_refuse_bad_arguments(L):
     assert lib.sr_grad_scale(0, 0, None, 0, 4096, None) == 0
     assert lib.sr_upload(4096, 4096, 6, None) == ARG and lib.sr_upload(None, 4096, 8, None) == ARG and lib.sr_upload(4096, 4098, 8, None) == ARG
     assert lib.sr_upload(None, None, 0, None) == 0
+    for src, dst, n, done in ((4096, 4096, 6, 4096), (None, 4096, 8, 4096), (4096, None, 8, 4096), (4100, 4096, 8, 4096), (4096, 4100, 8, 4096),
+                              (4096, 4096, 1 << 31, 4096), (4096, 4096, 0, 4096), (4096, 4096, 8, None), (4096, 4096, 8, 4100)):
+        assert lib.sr_upload_pinned(src, dst, n, done, 1, None) == ARG
 
 
 def test_python_refusals(L):

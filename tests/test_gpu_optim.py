@@ -141,10 +141,10 @@ def test_step_against_64_bits(T):
     assert (ep <= 3.5 * U * np.abs(p) + 12 * U * upd + slack).all()
 
 
-@pytest.mark.parametrize('bits', [32, 8])
-def test_missing_gradients_keep_their_own_count(T, bits):
+@pytest.mark.parametrize('bits,times', [(32, 1), (8, 1), (32, 200)])
+def test_missing_gradients_keep_their_own_count(T, bits, times):
     """A parameter without a gradient is skipped and its step count stays, as in torch.optim.AdamW; its average goes on."""
-    sizes = [300, 5, 2000, 64]
+    sizes = [300, 5, 2000, 64] * times
     arrays, grads = inputs(sizes, 31)
     params = [nn.Parameter(f32(a)) for a in arrays]
     opt = T.AdamW(params, state_bits=bits, ema_decay=0.5, **HP)
@@ -152,6 +152,7 @@ def test_missing_gradients_keep_their_own_count(T, bits):
     twin = [nn.Parameter(torch.from_numpy(a.astype(np.float64))) for a in arrays]
     topt = torch.optim.AdamW(twin, **HP)
     for have in ([1, 1, 0, 1], [0, 0, 0, 0], [1, 0, 0, 1], [1, 1, 1, 1], [1, 1, 1, 1], [0, 1, 1, 0]):
+        have = have * times
         gs = [g if h else None for g, h in zip(grads(), have)]
         for p, q, g in zip(params, twin, gs):
             p.grad = None if g is None else f32(g)
@@ -165,7 +166,7 @@ def test_missing_gradients_keep_their_own_count(T, bits):
         same(p, ref.p[i], 'p[%d]' % i)
     same(opt.ema, np.concatenate(ref.ema), 'ema')
     sd = opt.state_dict()
-    assert [int(sd['state'][i]['step']) for i in range(4)] == ref.t == [4, 4, 3, 4]
+    assert [int(sd['state'][i]['step']) for i in range(4 * times)] == ref.t == [4, 4, 3, 4] * times
     if bits == 32:   # six steps of order 1e-2 on values of order 4: 16 roundings of 2^-24 each
         for p, q in zip(params, twin):
             assert np.abs(p.detach().cpu().numpy() - q.detach().numpy()).max() <= 6 * 16 * U * 5
