@@ -464,7 +464,11 @@ def run_train(args, world, rank, dev, dist):
     sr, wf = sr.to(dev), wf.to(dev)
     # Adam over one flat buffer (same update rule as torch.optim.Adam(lr=1e-4) of the owner script; tests/test_cpu_host.py):
     # one gather, one all-reduce, five tensor ops per step instead of a walk over ~6000 parameter tensors
-    opt = T.FlatAdam(net.parameters(), lr=1e-4)
+    # (--optimizer adamw / adamw8: train.AdamW, one kernel over the tensors where they are, moments in float32 or 8 bits)
+    if args.optimizer == 'flat-adam':
+        opt = T.FlatAdam(net.parameters(), lr=1e-4)
+    else:
+        opt = T.AdamW(net.parameters(), lr=1e-4, state_bits=8 if args.optimizer == 'adamw8' else 32)
     # "L1 + perceptual".  Perceptual term as SURVEY 8(d) cfg4 prescribes: VGG19-shaped extractor, seeded
     # random initialisation (pretrained weights are a network fetch), features before ReLU at conv{1_2,2_2,3_4,4_4,5_4} with
     # weights {0.1,0.1,1,1,1} (options/train_realesrgan_x4plus.yml:133-149); --train-loss l1 = the owner script's loss alone
@@ -501,10 +505,12 @@ def run_train(args, world, rank, dev, dist):
         'warmup': max(args.warmup, 1), 'ms_per_step': step_s * 1e3, 'higher_is_better': True, 'scaling': 'weak',
         'vs_baseline': None, 'dtype': 'bf16' if mixed else 'f32', 'data': 'synthetic',
         'config': {'workload': 'training step of RRDBNet-FDConv(1,1,64,23,32): %d HR crops of %dx%d per GPU (LR %dx%d), train-mode '
-                               'forward + %s loss + backward + gradient all-reduce + Adam (train.FlatAdam: one flat buffer), %s '
+                               'forward + %s loss + backward + gradient all-reduce + %s, %s '
                                '(BASELINE.json configs[3])'
                                % (B, hr, hr, lr_side, lr_side,
                                   'bilinear/L1 + perceptual (seeded random-init VGG19 features, yml weights)' if perc else 'bilinear/L1 (owner script)',
+                                  {'flat-adam': 'Adam (train.FlatAdam: one flat buffer)', 'adamw': 'train.AdamW',
+                                   'adamw8': 'train.AdamW with 8-bit moments'}[args.optimizer],
                                   'bf16 activations on MFMA, float32 parameters / weight gradients / Adam' if mixed else 'float32'),
                    'global_batch': world * B, 'samples_per_s': world * B / step_s,
                    'parallelism': 'data parallel x%d, one all-reduce over the flat %.1f M-parameter gradient buffer per step (local BatchNorm statistics)' % (world, nparam / 1e6),
@@ -527,6 +533,7 @@ def main():
     ap.add_argument('--train-batch', type=int, default=32, help='train: HR crops per GPU and step')
     ap.add_argument('--train-hr', type=int, default=256, help='train: side of the HR crops')
     ap.add_argument('--train-dtype', choices=('bf16', 'f32'), default='bf16', help='train: bf16 = mixed precision (bf16 activations on the matrix cores, float32 parameters and weight gradients); f32 = the parity path')
+    ap.add_argument('--optimizer', choices=('flat-adam', 'adamw', 'adamw8'), default='flat-adam', help='train: train.FlatAdam, or train.AdamW with float32 / 8-bit moments')
     ap.add_argument('--train-loss', choices=('l1+perceptual', 'l1'), default='l1+perceptual', help='train: BASELINE configs[3] says L1 + perceptual; l1 = the owner script (train_realESRGAN_fdconv_1.py:116)')
     ap.add_argument('--batch', type=int, default=16)
     ap.add_argument('--size', type=int, default=512)

@@ -351,8 +351,8 @@ class AdamW(torch.optim.Optimizer):
     kernel); `ema_parameters()` gives it tensor by tensor, for a `params_ema` checkpoint.
     clip_grad_norm in step(): the global norm of all gradients, its factor applied as the gradients are read (they are not
     written back); `opt.grad_norm` holds the norm afterwards, on the device.  Nothing in step() waits for the GPU.
-    In a process group of more than one rank step() all-reduces the gradients first (train.allreduce_gradients), and the
-    constructor broadcasts rank 0's parameters (`broadcast=False`: not).
+    In a process group of more than one rank step() all-reduces the gradients first (train.allreduce_gradients: a missing one
+    counts as zeros), and the constructor broadcasts rank 0's parameters (`broadcast=False`: not).
 
     Parameters without a gradient are skipped, with their own step count, as torch does; their average goes on.
     state_dict() / load_state_dict() use torch.optim.AdamW's layout (float32 `exp_avg`, `exp_avg_sq`, `step`; plus `ema`), so a
