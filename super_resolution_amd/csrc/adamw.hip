@@ -542,10 +542,10 @@ __global__ __launch_bounds__(256) void adamw_set_moments_kernel(const Rec* __res
 // ---- global gradient norm ---------------------------------------------------------------------------------------------
 // Squares are added in float64 (a float32 square overflows from 1.8e19 on, and 1e8 of them lose three digits; float64 multiply-adds
 // run at the float32 rate here), in an order that the shapes alone determine.  Work items are runs of consecutive values; waves
-// take them in turn, four 16-byte loads of every lane in flight (256 M bfloat16 values: norm 0.10 ms, 5 TB/s; scaling 0.18 ms, 5.8
-// TB/s, 0.21 with one 8-byte load at a time; both 0.27, and 0.29 if the scaling does not go backwards).  Right after a step the norm of 48 M bfloat16 values takes 37 us instead of 25: the
-// memory-side cache is full of what the step wrote, and every line read pushes one out.  Two or four pieces at a time did not
-// change that.
+// take them in turn, four 16-byte loads of every lane in flight.  256 M bfloat16 values: norm 0.10 ms, 5 TB/s; scaling 0.18 ms, 5.8
+// TB/s (0.21 with one 8-byte load at a time); both 0.27, and 0.29 if the scaling does not go backwards.  Right after a step the
+// norm of 48 M bfloat16 values takes 37 us instead of 25: the memory-side cache is full of what the step wrote, and every line read
+// pushes one out.  Two or four pieces at a time did not change that.
 template <typename G>
 struct PieceSource {  // the pieces of an optimizer's list, gradients by tensor
     const Rec* recs;
