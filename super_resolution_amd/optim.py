@@ -380,6 +380,8 @@ class AdamW(torch.optim.Optimizer):
             if not _is_dense(p):
                 raise ValueError('AdamW: a parameter with holes or repeated elements')
         self._check_overlap()
+        # shape, strides and order of the elements that moments and average are kept in
+        self._layout = [self._layout_now(p) for p in self.params]
         # places: element number among all parameters; offset among the tensors of the same kind of moments; first block
         size = np.array([p.numel() for p in self.params], dtype=np.int64)
         bits = np.repeat([g['state_bits'] for g in self.param_groups], [len(g['params']) for g in self.param_groups])
@@ -456,10 +458,14 @@ class AdamW(torch.optim.Optimizer):
                 return torch._utils._flatten_dense_tensors(tensors)    # one C++ call for thousands of tensors
             return torch.cat([t.as_strided((t.numel(),), (1,)).float() for t in tensors])
 
+    @staticmethod
+    def _layout_now(p):
+        return p.shape, p.stride(), p.is_contiguous()
+
     def _shaped(self, flat, i):
-        """Tensor i's part of a flat array, in the parameter's shape and strides."""
-        p, at = self.params[i], int(self._index[i])
-        return flat[at:at + p.numel()].as_strided(p.shape, p.stride())
+        """Tensor i's part of a flat array, with its elements at the parameter's indices."""
+        at, (shape, stride, _) = int(self._index[i]), self._layout[i]
+        return flat[at:at + shape.numel()].as_strided(shape, stride)
 
     @property
     def exp_avg(self):
@@ -564,13 +570,50 @@ class AdamW(torch.optim.Optimizer):
 
     def _follow(self, lst, capturing):
         """Parameters lie elsewhere (`.data =`): same dtype, device and size are followed, anything else is refused."""
-        for p, n in zip(lst.params, lst.sizes):
-            if p.device != self.device or p.dtype != lst.dtype or p.numel() != n or not _is_dense(p):
+        turned = []
+        for i, p in zip(lst.members, lst.params):
+            shape, stride, contiguous = self._layout[i]
+            if p.device != self.device or p.dtype != lst.dtype or p.shape != shape or not _is_dense(p):
                 raise RuntimeError('AdamW: a parameter was moved, cast or resized after the optimizer was built -- rebuild the optimizer')
+            if p.stride() != stride and not (contiguous and p.is_contiguous()):
+                turned.append(i)
         if capturing:
             raise RuntimeError('AdamW: a parameter was re-pointed; run one step outside the capture first')
         self._check_overlap()
+        for i in turned:
+            self._reorder(i, lst.bits)
         lst.build(self)
+
+    @torch.no_grad()
+    def _reorder(self, i, bits):
+        """The memory order of parameter i has changed (channels_last and back): its moments and its average follow, so that every
+        element keeps its own.  Blocks of 8-bit moments then hold other elements, and these are rounded once more."""
+        p, n = self.params[i], self.params[i].numel()
+        shape, stride, _ = self._layout[i]
+        index, at, block = int(self._index[i]), int(self._at[i]), int(self._block[i])
+
+        def turn(x):
+            x.as_strided(p.shape, p.stride()).copy_(x.clone().as_strided(shape, stride))
+        if bits == 32:
+            turn(self._m32[at:at + n])
+            turn(self._v32[at:at + n])
+        else:
+            t, h, lib, st = (L.AdamWTensor * 1)(), C.c_void_p(), L.lib(), _stream(self.device)
+            t[0].p, t[0].n = p.data_ptr(), n
+            t[0].m, t[0].v = self._m8.data_ptr() + at, self._v8.data_ptr() + at
+            t[0].me, t[0].ve = self._me.data_ptr() + block, self._ve.data_ptr() + block
+            L.check(lib.sr_adamw_create(L.dtype_code(p.dtype), 8, 1, t, C.byref(h)), 'sr_adamw_create')
+            try:
+                m, v = (torch.empty(n, dtype=torch.float32, device=self.device) for _ in range(2))
+                L.check(lib.sr_adamw_moments(h, L.SR_F32, m.data_ptr(), v.data_ptr(), st), 'sr_adamw_moments')
+                turn(m)
+                turn(v)
+                L.check(lib.sr_adamw_set_moments(h, m.data_ptr(), v.data_ptr(), self.seed, st), 'sr_adamw_set_moments')
+            finally:
+                lib.sr_adamw_destroy(h)
+        if self.ema is not None:
+            turn(self.ema[index:index + n])
+        self._layout[i] = self._layout_now(p)
 
     def _check_overlap(self):
         spans = np.array([(p.data_ptr(), p.numel() * p.element_size()) for p in self.params if p.numel()], dtype=np.int64).reshape(-1, 2)
@@ -630,9 +673,9 @@ class AdamW(torch.optim.Optimizer):
         state = {place[k]: s for k, s in sd['state'].items()}
         for i, s in state.items():
             for name in ('exp_avg', 'exp_avg_sq', 'ema'):
-                if name in s and s[name].shape != self.params[i].shape:
+                if name in s and s[name].shape != self._layout[i][0]:
                     raise ValueError('AdamW.load_state_dict: parameter %d has shape %s, its %s %s'
-                                     % (i, tuple(self.params[i].shape), name, tuple(s[name].shape)))
+                                     % (i, tuple(self._layout[i][0]), name, tuple(s[name].shape)))
         new = [{k: g.get(k, mine[k]) for k in ('lr', 'betas', 'eps', 'weight_decay')} for g, mine in zip(groups, self.param_groups)]
         for hp in new:
             self._hyper(hp)
@@ -643,12 +686,13 @@ class AdamW(torch.optim.Optimizer):
             mine.update(hp)
 
         def part(name, i):
-            p, x = self.params[i], state.get(i, {}).get(name)
+            shape, stride, _ = self._layout[i]
+            x = state.get(i, {}).get(name, self.params[i] if name == 'ema' else None)
             if x is None:
-                return torch.zeros(p.numel(), dtype=torch.float32, device=self.device) if name != 'ema' else p.float()
+                return torch.zeros(shape.numel(), dtype=torch.float32, device=self.device)
             if x.dtype != torch.float32 or x.device != self.device:
                 x = x.to(self.device, torch.float32)
-            return x if x.stride() == p.stride() else torch.empty_like(p, dtype=torch.float32).copy_(x)
+            return x if x.stride() == stride else torch.empty_strided(shape, stride, dtype=torch.float32, device=self.device).copy_(x)
 
         def flat(name):
             return self._cat([part(name, i) for i in range(len(self.params))])

@@ -1,0 +1,56 @@
+"""AdamW / clip_grad_norm_ in the calls around a training loop, without a GPU: re-pointed parameters as the host walk sees them,
+arguments by position, version counters."""
+import ctypes as C
+import inspect
+
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+
+@pytest.fixture(scope='module')
+def host():
+    from super_resolution_amd.build import build
+    build(verbose=False)
+    from super_resolution_amd import optim
+    return optim._host_lib()
+
+
+def _track(host, tensors):
+    h = host.srt_track(tensors)
+    assert h
+    n = len(tensors)
+    ptr, odd, nodd, moved = (C.c_uint64 * n)(), (C.c_int64 * n)(), C.c_int64(), C.c_int64()
+
+    def walk():
+        missing = host.srt_gradients(h, ptr, odd, C.byref(nodd), C.byref(moved))
+        return missing, nodd.value, moved.value
+    return h, walk
+
+
+def test_walk_sees_another_memory_order(host):
+    """Strides at the same address, and another storage at the same address; strides of dimensions of one element are no order."""
+    memory = np.zeros(24, np.float32)
+    ps = [nn.Parameter(torch.zeros(s)) for s in ((4, 8, 3, 3), (12, 12), (6, 4), (5, 1, 1, 7))]
+    ps[2].data = torch.from_numpy(memory).view(6, 4)
+    h, walk = _track(host, ps)
+    assert walk() == (4, 0, 0)
+    ps[1].data = ps[1].data.t()
+    assert walk() == (4, 0, 1)
+    ps[1].data = ps[1].data.t()
+    assert walk() == (4, 0, 0)
+    ps[3].data = ps[3].data.as_strided((5, 1, 1, 7), (7, 1, 99, 1))
+    assert walk() == (4, 0, 0)
+    ps[2].data = ps[2].data.view(4, 6)
+    assert walk() == (4, 0, 0)          # every element is where it was
+    ps[2].data = torch.from_numpy(memory).view(4, 6)
+    assert walk() == (4, 0, 1)          # memory that was given back and taken again
+    ps[0].data = ps[0].data.to(memory_format=torch.channels_last)
+    assert walk() == (4, 0, 2)
+    h2, walk2 = _track(host, ps[:1])
+    assert walk2() == (1, 0, 0)
+    ps[0].data = ps[0].data.as_strided((4, 8, 3, 3), (72, 9, 3, 1))
+    assert walk2() == (1, 0, 1)
+    host.srt_untrack(h2)
+    host.srt_untrack(h)

@@ -1,0 +1,126 @@
+"""train.AdamW and train.clip_grad_norm_ in the calls around a training loop: re-pointed parameters, schedulers and checkpoints, captured
+steps beside evaluation, many groups, gradients that share memory.
+
+As in test_gpu_optim.py float32 results are compared bit for bit with the formulas of tests/adamw_ref.py."""
+import copy
+
+import numpy as np
+import pytest
+import torch
+import torch.nn as nn
+
+import adamw_ref as R
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24      # largest relative error of one float32 rounding
+HP = dict(lr=1e-2, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.1)
+
+
+@pytest.fixture(scope='module')
+def T():
+    from super_resolution_amd import _lib, train
+    _lib.lib()
+    assert torch.cuda.is_available()
+    return train
+
+
+def f32(x):
+    return torch.from_numpy(np.ascontiguousarray(x)).cuda()
+
+
+def same(got, want, what):
+    """Bit for bit (NaN as NaN), in the order of the indices, whatever the strides."""
+    got, want = got.detach().float().cpu().contiguous().numpy().reshape(-1), np.asarray(want).reshape(-1)
+    assert got.shape == want.shape, what
+    bad = ~((got == want) | (np.isnan(got) & np.isnan(want)))
+    assert not bad.any(), '%s: %d of %d differ, first %d: %r, reference %r' % (what, bad.sum(), bad.size, bad.argmax(), got[bad.argmax()], want[bad.argmax()])
+
+
+# ---- parameters whose memory order changes -------------------------------------------------------------------------------
+ORDERS = {
+    'channels_last': ((4, 8, 3, 3), lambda x: x.to(memory_format=torch.channels_last)),
+    'contiguous again': ((4, 8, 3, 3), lambda x: x.contiguous()),
+    'transposed memory': ((40, 60), lambda x: x.t().contiguous().t()),
+    'transposed at the same address': ((24, 24), lambda x: x.t()),
+}
+
+
+@pytest.mark.parametrize('name', list(ORDERS))
+@pytest.mark.parametrize('capturable', [False, True])
+def test_another_memory_order_keeps_every_elements_moments(T, name, capturable):
+    """Element (i, j, ...) keeps its moments and its average, as in torch.optim.AdamW."""
+    shape, turn = ORDERS[name]
+    rng = np.random.default_rng(5)
+    a, b = rng.standard_normal(shape).astype(np.float32), rng.standard_normal(50).astype(np.float32)
+    p, q = nn.Parameter(f32(a)), nn.Parameter(f32(b))
+    if name == 'contiguous again':
+        p.data = p.data.to(memory_format=torch.channels_last)
+    opt = T.AdamW([q, p], ema_decay=0.9, capturable=capturable, **HP)
+    ref = R.Tensors([b, a.reshape(-1)], dict(HP, ema=0.9))
+
+    def go():
+        gs = [rng.standard_normal(50).astype(np.float32), rng.standard_normal(shape).astype(np.float32)]
+        q.grad, p.grad = f32(gs[0]), f32(gs[1])
+        opt.step()
+        ref.step([g.reshape(-1) for g in gs])
+
+    def check(what):
+        same(p, ref.p[1], 'p, ' + what)
+        same(q, ref.p[0], 'q, ' + what)
+        state = opt.state_dict()['state']
+        for i in range(2):
+            same(state[i]['exp_avg'], ref.m[i], 'm[%d], %s' % (i, what))
+            same(state[i]['exp_avg_sq'], ref.v[i], 'v[%d], %s' % (i, what))
+            same(state[i]['ema'], ref.ema[i], 'ema[%d], %s' % (i, what))
+            same(opt.ema_parameters()[i], ref.ema[i], 'ema_parameters[%d], %s' % (i, what))
+    go()
+    go()
+    check('before')
+    p.data = turn(p.data)
+    ref.p[1] = p.detach().cpu().contiguous().numpy().reshape(-1)     # (the transposed one has other values at its indices)
+    check('re-pointed')
+    saved = copy.deepcopy(opt.state_dict())
+    go()
+    go()
+    check('stepped')
+    opt.load_state_dict(saved)       # the dictionary goes by index, not by memory
+    for i, s in opt.state_dict()['state'].items():
+        assert all(torch.equal(s[k], saved['state'][i][k]) for k in ('exp_avg', 'exp_avg_sq', 'ema'))
+
+
+def test_another_memory_order_with_8_bit_moments(T):
+    """The moments are rounded once more on the way.  Gradients 2^(i % 5): all codes in the normal range, where one rounding moves a value
+    by less than its eighth; so two of them (the way and the step with zero gradients after it) by a factor within (1 - 1/8)^2 and
+    (1 + 1/8)^2.  Neighbours differ by a factor of two at least."""
+    shape = (8, 16, 3, 3)
+    n = int(np.prod(shape))
+    g = (2.0 ** (np.arange(n) % 5)).astype(np.float32).reshape(shape)
+    p, q = nn.Parameter(torch.ones(shape, device='cuda')), nn.Parameter(torch.ones(300, device='cuda'))
+    opt = T.AdamW([p, q], state_bits=8, ema_decay=0.9, **HP)
+    for _ in range(3):
+        p.grad, q.grad = f32(g), torch.ones(300, device='cuda')
+        opt.step()
+    m, v = (opt.state_dict()['state'][0][k].cpu().numpy() for k in ('exp_avg', 'exp_avg_sq'))
+    ema, other = opt.ema_parameters()[0].cpu().numpy(), opt.state_dict()['state'][1]['exp_avg'].clone()
+    p.data = p.data.to(memory_format=torch.channels_last)
+    p.grad, q.grad = torch.zeros_like(p), None
+    opt.step()
+    s = opt.state_dict()['state']
+    lo, hi = (1 - 1 / 8) ** 2, (1 + 1 / 8) ** 2
+    r = s[0]['exp_avg'].cpu().numpy() / (np.float32(0.9) * m)
+    assert lo <= r.min() and r.max() <= hi, (r.min(), r.max())
+    r = s[0]['exp_avg_sq'].cpu().numpy() / (np.float32(0.999) * v)
+    assert lo <= r.min() and r.max() <= hi, (r.min(), r.max())
+    want = ema * np.float32(0.9) + p.detach().cpu().numpy() * np.float32(1 - 0.9)
+    same(opt.ema_parameters()[0], want, 'ema')
+    assert torch.equal(s[1]['exp_avg'], other)
+
+
+def test_another_shape_is_refused(T):
+    p = nn.Parameter(torch.randn(6, 4, device='cuda'))
+    opt = T.AdamW([p], **HP)
+    for x in (p.data.t().contiguous(), p.data.clone().view(-1)):
+        p.data = x
+        p.grad = torch.zeros_like(p)
+        with pytest.raises(RuntimeError, match='rebuild'):
+            opt.step()
