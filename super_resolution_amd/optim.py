@@ -154,14 +154,17 @@ def _world(group):
 # ------------------------------------------------------------------------------------------------------------------
 # clipping
 # ------------------------------------------------------------------------------------------------------------------
-def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
-    """torch.nn.utils.clip_grad_norm_ (2-norm): scales the gradients in place by min(1, max_norm / (norm + 1e-6)) and returns the
-    norm, a 0-d float32 tensor.  Squares are summed in float64, in an order that the shapes alone determine; nothing waits for
-    the GPU unless error_if_nonfinite is set.  float32 and bfloat16 gradients, mixed, on one GPU."""
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ for the 2-norm (any other norm_type raises): scales the gradients in place by
+    min(1, max_norm / (norm + 1e-6)) and returns the norm, a 0-d float32 tensor.  Squares are summed in float64, in an order that
+    the shapes alone determine; nothing waits for the GPU unless error_if_nonfinite is set.  float32 and bfloat16 gradients, mixed,
+    on one GPU."""
     params = [parameters] if torch.is_tensor(parameters) else list(parameters)
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError('clip_grad_norm_: max_norm must not be negative (got %r)' % max_norm)
+    if isinstance(norm_type, bool) or float(norm_type) != 2:
+        raise ValueError('clip_grad_norm_: norm_type is 2 (got %r)' % (norm_type,))
     host, lib = _host_lib(), L.lib()
     device, counts = C.c_int(-1), (C.c_int64 * 3)()
     rc = host.srt_spans(params, 1, C.byref(device), counts)

@@ -54,3 +54,15 @@ def test_walk_sees_another_memory_order(host):
     assert walk2() == (1, 0, 1)
     host.srt_untrack(h2)
     host.srt_untrack(h)
+
+
+def test_clip_takes_torchs_arguments_in_torchs_order():
+    from super_resolution_amd import train
+    theirs = list(inspect.signature(torch.nn.utils.clip_grad_norm_).parameters)[:4]
+    assert list(inspect.signature(train.clip_grad_norm_).parameters)[:4] == theirs
+    p = nn.Parameter(torch.zeros(4))
+    for other in (1.0, 1, float('inf'), 0.0, 3.0, True):
+        with pytest.raises(ValueError, match='norm_type'):
+            train.clip_grad_norm_([p], 1.0, other)
+    for two in (2.0, 2, '2'):
+        assert float(train.clip_grad_norm_([p], 1.0, two)) == 0.0

@@ -124,3 +124,17 @@ def test_another_shape_is_refused(T):
         p.grad = torch.zeros_like(p)
         with pytest.raises(RuntimeError, match='rebuild'):
             opt.step()
+
+
+# ---- clipping ------------------------------------------------------------------------------------------------------------
+def test_clip_arguments_by_position(T):
+    p = nn.Parameter(torch.zeros(3, device='cuda'))
+    p.grad = torch.tensor([float('inf'), 1.0, 2.0], device='cuda')
+    assert float(T.clip_grad_norm_(p, 1e30, 2.0)) == float('inf')        # the norm's type, not error_if_nonfinite
+    p.grad = torch.tensor([float('inf'), 1.0, 2.0], device='cuda')
+    with pytest.raises(RuntimeError, match='finite'):
+        T.clip_grad_norm_(p, 1.0, 2.0, True)
+    p.grad = torch.tensor([3.0, 4.0, 0.0], device='cuda')
+    with pytest.raises(ValueError, match='norm_type'):
+        T.clip_grad_norm_(p, 1.0, float('inf'))
+    assert p.grad.tolist() == [3.0, 4.0, 0.0]
