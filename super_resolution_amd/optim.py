@@ -169,20 +169,20 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     device, counts = C.c_int(-1), (C.c_int64 * 3)()
     rc = host.srt_spans(params, 1, C.byref(device), counts)
     odd = []
-    if rc <= -2:   # gradients with holes (or expanded ones): the norm reads dense copies, torch scales the originals
-        grads = [p.grad for p in params if p.grad is not None]
-        dense = []
-        for g in grads:
-            c = g if _is_dense(g) else g.detach().contiguous()
-            if c is not g:
-                odd.append(g)
-            dense.append(c)
+    if rc <= -2:   # gradients with holes: the norm reads dense copies, torch scales the originals
+        grads = [(i, p.grad) for i, p in enumerate(params) if p.grad is not None]
+        for i, g in grads:
+            if g.layout != torch.strided or g.dtype not in (torch.float32, torch.bfloat16) or not g.is_cuda or g.device != grads[0][1].device:
+                raise _unfit(i)
+        _check_separate(grads)
+        odd = [g for _, g in grads if not _is_dense(g)]
+        dense = [g if _is_dense(g) else g.detach().contiguous() for _, g in grads]      # (alive until the norm is launched)
         device = C.c_int(-1)
         rc = host.srt_spans(dense, 0, C.byref(device), counts)
     if rc == -1:
         _host_failed('clip_grad_norm_')
     if rc > 0:
-        raise TypeError('clip_grad_norm_: gradients are float32 or bfloat16 on one GPU; tensor %d is not' % (rc - 1))
+        raise _unfit(rc - 1)
     if not counts[2]:
         return torch.tensor(0.0)
     dev = torch.device('cuda', device.value)
@@ -219,6 +219,47 @@ def _is_dense(t):
             return False
         n *= size
     return True
+
+
+def _unfit(i):
+    return TypeError('clip_grad_norm_: gradients are float32 or bfloat16 on one GPU; tensor %d is not' % i)
+
+
+def _extent(t):
+    """The bytes between which the tensor lies: (first, behind the last)."""
+    return t.data_ptr(), t.data_ptr() + ((sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else 0)
+
+
+def _claimed_twice(tensors):
+    """Whether tensors with overlapping extents, of any strides, have an element's memory in common, or one of them has it twice: every
+    pair of bytes is marked."""
+    first = min(_extent(t)[0] for t in tensors)
+    mark, claims = np.zeros((max(_extent(t)[1] for t in tensors) - first) // 2, dtype=bool), 0
+    for t in tensors:
+        k = t.element_size() // 2
+        at = (t.data_ptr() - first) // 2
+        np.lib.stride_tricks.as_strided(mark[at:], tuple(t.shape) + (k,), tuple(s * k for s in t.stride()) + (1,))[...] = True
+        claims += t.numel() * k
+    return int(np.count_nonzero(mark)) != claims
+
+
+def _check_separate(grads):
+    """Refuses gradients (numbered; not all dense) that scaling in place would scale twice."""
+    grads = [(i, g) for i, g in grads if g.numel()]
+    for i, g in grads:
+        reach = 0     # elements that the smaller strides reach: beyond them nothing repeats
+        for s, n in sorted((s, n) for n, s in zip(g.shape, g.stride()) if n != 1):
+            if s <= reach and _claimed_twice([g]):
+                raise RuntimeError('clip_grad_norm_: the gradient of tensor %d repeats its elements: it cannot be scaled in place' % i)
+            reach += (n - 1) * s
+    cluster, end = [], 0
+    for (lo, hi), g in sorted(((_extent(g), g) for _, g in grads), key=lambda x: x[0]) + [((float('inf'), 0), None)]:
+        if lo >= end:
+            if len(cluster) > 1 and _claimed_twice(cluster):
+                raise RuntimeError('clip_grad_norm_: two gradients share memory')
+            cluster, end = [], 0
+        cluster.append(g)
+        end = max(end, hi)
 
 
 def _norm(lists, max_norm, dev, st):

@@ -66,3 +66,36 @@ def test_clip_takes_torchs_arguments_in_torchs_order():
             train.clip_grad_norm_([p], 1.0, other)
     for two in (2.0, 2, '2'):
         assert float(train.clip_grad_norm_([p], 1.0, two)) == 0.0
+
+
+def test_shared_elements_against_a_list_of_all_bytes():
+    """Random strided views of one block of memory, float32 and bfloat16 mixed: refused exactly where two bytes' claims meet."""
+    import random
+    from super_resolution_amd import optim
+
+    def claimed_twice(tensors):
+        seen = set()
+        for t in tensors:
+            for index in np.ndindex(*t.shape):
+                at = t.data_ptr() + sum(i * s for i, s in zip(index, t.stride())) * t.element_size()
+                pairs = range(at, at + t.element_size(), 2)
+                if any(b in seen for b in pairs):
+                    return True
+                seen.update(pairs)
+        return False
+    rng, found = random.Random(1), [0, 0]
+    buf = torch.zeros(400)
+    for _ in range(600):
+        views = []
+        for _ in range(rng.choice((1, 2, 3))):
+            dims = rng.randrange(4)
+            views.append(rng.choice((buf, buf.view(torch.bfloat16))).as_strided([rng.randrange(5) for _ in range(dims)],
+                                                                              [rng.choice((0, 1, 1, 2, 3, 4, 6, 8, 12)) for _ in range(dims)], rng.randrange(60)))
+        want = claimed_twice(views)
+        found[want] += 1
+        if want:
+            with pytest.raises(RuntimeError, match='repeats|share'):
+                optim._check_separate(list(enumerate(views)))
+        else:
+            optim._check_separate(list(enumerate(views)))
+    assert min(found) > 100

@@ -138,3 +138,59 @@ def test_clip_arguments_by_position(T):
     with pytest.raises(ValueError, match='norm_type'):
         T.clip_grad_norm_(p, 1.0, float('inf'))
     assert p.grad.tolist() == [3.0, 4.0, 0.0]
+
+
+@pytest.mark.parametrize('name', ['the same tensor', 'two views alike', 'columns of each other', 'a dense one over a strided one', 'one parameter twice'])
+def test_clip_refuses_shared_memory_in_any_layout(T, name):
+    """A gradient that would be scaled twice is refused before anything is written."""
+    whole = torch.ones(6, 16, device='cuda')
+    ps = [nn.Parameter(torch.zeros(s, device='cuda')) for s in ((6, 8), (6, 8), (7,))]
+    ps[2].grad = torch.full((7,), 3.0, device='cuda')
+    ps[0].grad = whole[:, ::2]
+    if name == 'the same tensor':
+        ps[1].grad = ps[0].grad
+    elif name == 'two views alike':
+        ps[1].grad = whole[:, ::2]
+    elif name == 'columns of each other':
+        ps[1].grad = whole[:, :8]
+    elif name == 'a dense one over a strided one':
+        ps[1].grad = whole[:3].view(6, 8)
+    else:
+        ps.append(ps[0])
+    with pytest.raises(RuntimeError, match='share'):
+        T.clip_grad_norm_(ps, 1.0)
+    assert bool((whole == 1).all()) and bool((ps[2].grad == 3).all())
+
+
+def test_clip_refuses_repeated_elements(T):
+    """Expanded gradients, and windows that slide, cannot be scaled in place (torch raises too): refused before anything is written."""
+    for g in (torch.ones(6, 1, device='cuda').expand(6, 8), torch.ones(60, device='cuda').as_strided((6, 8), (3, 1))):
+        ps = [nn.Parameter(torch.zeros(s, device='cuda')) for s in ((7,), (2,), (6, 8))]
+        ps[0].grad, ps[2].grad = torch.full((7,), 3.0, device='cuda'), g
+        with pytest.raises(RuntimeError, match='tensor 2.*repeat'):
+            T.clip_grad_norm_(ps, 1.0)
+        assert bool((g == 1).all()) and bool((ps[0].grad == 3).all())
+
+
+def test_clip_of_interleaved_gradients(T):
+    """Views that lie between each other without sharing an element are scaled like any others."""
+    whole, half = torch.ones(6, 16, device='cuda'), torch.ones(4, 6, 2, device='cuda', dtype=torch.bfloat16)
+    ps = [nn.Parameter(torch.zeros(s, device='cuda', dtype=d)) for s, d in (((6, 8), torch.float32), ((6, 8), torch.float32), ((7,), torch.float32),
+                                                                           ((4, 6), torch.bfloat16), ((4, 6), torch.bfloat16))]
+    for p, g in zip(ps, (whole[:, ::2], whole[:, 1::2], torch.full((7,), 3.0, device='cuda'), half[..., 0], half[..., 1])):
+        p.grad = g
+    want = (96 + 9 * 7 + 48) ** 0.5
+    assert abs(float(T.clip_grad_norm_(ps, 1.0)) - want) <= 2 * U * want
+    f = np.float32(1.0 / (want + 1e-6))
+    assert bool((whole == float(f)).all()) and bool((ps[2].grad == float(np.float32(3) * f)).all())
+    assert bool((half == torch.tensor(f).bfloat16().cuda()).all())
+
+
+def test_clip_names_the_parameter_that_does_not_fit(T):
+    """Counted among the parameters, also where one has no gradient and another one is not dense."""
+    ps = [nn.Parameter(torch.zeros(4, 3, device='cuda', dtype=d)) for d in (torch.float32, torch.float32, torch.float16)]
+    whole = torch.ones(4, 6, device='cuda')
+    ps[1].grad, ps[2].grad = whole[:, ::2], torch.ones(4, 3, device='cuda', dtype=torch.float16)
+    with pytest.raises(TypeError, match='tensor 2'):
+        T.clip_grad_norm_(ps, 1.0)
+    assert bool((whole == 1).all())
