@@ -8,6 +8,7 @@ train/train_realESRGAN_fdconv.py:142, and the weight average that Real-ESRGAN ch
 one kernel (csrc/adamw.hip) walks all tensors of a group, reads gradients, parameters and moments once and writes them once.
 """
 import contextlib
+import copy
 import ctypes as C
 import os
 import threading
@@ -674,6 +675,9 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError('AdamW(capturable=True): a step must bring gradients for the same parameters as the one before')
 
     # ---- checkpoints ---------------------------------------------------------------------------------------------------
+    # group keys that belong to this optimizer's layout, or to the implementation that wrote the dictionary
+    _NOT_LOADED = ('params', 'state_bits', 'amsgrad', 'maximize', 'foreach', 'capturable', 'differentiable', 'fused', 'decoupled_weight_decay')
+
     def _steps_of(self, lst):
         if self.capturable:
             t = int(lst.step_dev.item())
@@ -709,6 +713,8 @@ class AdamW(torch.optim.Optimizer):
         for g in groups:
             if g.get('amsgrad') or g.get('maximize'):
                 raise ValueError('AdamW.load_state_dict: amsgrad and maximize are not supported')
+            if g.get('decoupled_weight_decay') is False and g.get('weight_decay'):
+                raise ValueError('AdamW.load_state_dict: the weight decay of torch.optim.Adam (part of the gradient) is not supported')
         place = {}
         for i, key in enumerate(k for g in groups for k in g['params']):
             place[key] = i
@@ -720,7 +726,9 @@ class AdamW(torch.optim.Optimizer):
                 if name in s and s[name].shape != self._layout[i][0]:
                     raise ValueError('AdamW.load_state_dict: parameter %d has shape %s, its %s %s'
                                      % (i, tuple(self._layout[i][0]), name, tuple(s[name].shape)))
-        new = [{k: g.get(k, mine[k]) for k in ('lr', 'betas', 'eps', 'weight_decay')} for g, mine in zip(groups, self.param_groups)]
+        # the rates, and what schedulers keep beside them
+        new = [{**{k: mine[k] for k in ('lr', 'betas', 'eps', 'weight_decay')}, **{k: copy.deepcopy(x) for k, x in g.items() if k not in self._NOT_LOADED}}
+               for g, mine in zip(groups, self.param_groups)]
         for hp in new:
             self._hyper(hp)
         steps = [np.array([int(float(state.get(i, {}).get('step', 0))) for i in lst.members], dtype=np.int64) for lst in self._lists]

@@ -194,3 +194,52 @@ def test_clip_names_the_parameter_that_does_not_fit(T):
     with pytest.raises(TypeError, match='tensor 2'):
         T.clip_grad_norm_(ps, 1.0)
     assert bool((whole == 1).all())
+
+
+# ---- checkpoints, schedulers ---------------------------------------------------------------------------------------------
+def _one(T, **kw):
+    p = nn.Parameter(torch.ones(300, device='cuda'))
+    return p, T.AdamW([p], **dict(dict(lr=1e-2), **kw))
+
+
+def test_a_scheduler_resumes(T):
+    """What a scheduler keeps in the groups (initial_lr, max_lr, ...) comes back with the checkpoint; what belongs to the layout or to
+    another optimizer's implementation does not."""
+    p, opt = _one(T)
+    sch = torch.optim.lr_scheduler.StepLR(opt, step_size=2, gamma=0.1)
+    p.grad = torch.ones_like(p)
+    for _ in range(3):
+        opt.step()
+        sch.step()
+    saved = copy.deepcopy(opt.state_dict())
+    _, again = _one(T, state_bits=8)
+    again.load_state_dict(saved)
+    assert again.param_groups[0]['initial_lr'] == 1e-2 and again.param_groups[0]['state_bits'] == 8
+    sch2 = torch.optim.lr_scheduler.StepLR(again, step_size=2, gamma=0.1, last_epoch=sch.last_epoch - 1)   # (the constructor takes a step)
+    p2 = again.params[0]
+    for _ in range(2):
+        p2.grad = torch.ones_like(p2)
+        opt.step()
+        again.step()
+        sch.step()
+        sch2.step()
+        assert abs(opt.param_groups[0]['lr'] - again.param_groups[0]['lr']) <= 1e-12
+    _, third = _one(T)
+    theirs = torch.optim.AdamW([nn.Parameter(torch.ones(300))], lr=3e-4)
+    third.load_state_dict(theirs.state_dict())
+    assert third.param_groups[0]['lr'] == 3e-4 and 'fused' not in third.param_groups[0] and 'foreach' not in third.param_groups[0]
+    with pytest.raises(ValueError, match='decay'):      # Adam's decay is not this one
+        third.load_state_dict(torch.optim.Adam([nn.Parameter(torch.ones(300))], weight_decay=0.1).state_dict())
+    third.load_state_dict(torch.optim.Adam([nn.Parameter(torch.ones(300))], lr=2e-4).state_dict())
+    assert third.param_groups[0]['lr'] == 2e-4
+
+
+def test_loading_takes_copies(T):
+    p, opt = _one(T, betas=[0.9, 0.99])
+    opt.param_groups[0]['note'] = {'k': [1]}
+    saved = opt.state_dict()
+    _, other = _one(T)
+    other.load_state_dict(saved)
+    other.param_groups[0]['note']['k'].append(2)
+    other.param_groups[0]['betas'][1] = 0.5
+    assert opt.param_groups[0]['note'] == {'k': [1]} and list(opt.param_groups[0]['betas']) == [0.9, 0.99]
