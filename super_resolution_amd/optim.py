@@ -294,6 +294,7 @@ class _List:
         self.odd = (C.c_int64 * self.n)()
         self.nodd, self.moved = C.c_int64(), C.c_int64()
         self.seen = self.step_dev = self.scalars = None
+        self.rates = []             # learning rates on the device that captured steps read
         if opt.capturable:          # fixed memory: captured graphs point to it
             self.step_dev = torch.zeros((), dtype=torch.int64, device=opt.device)
             self.scalars = torch.empty(L.ADAMW_SCALARS_BYTES, dtype=torch.uint8, device=opt.device)
@@ -590,6 +591,8 @@ class AdamW(torch.optim.Optimizer):
             return
         if self.capturable:
             lr = self.param_groups[lst.group]['lr']
+            if torch.is_tensor(lr) and lr.is_cuda and torch.cuda.is_current_stream_capturing() and not any(lr is x for x in lst.rates):
+                lst.rates.append(lr)
             L.check(lib.sr_adamw_tick(C.byref(h), lr.data_ptr() if torch.is_tensor(lr) and lr.is_cuda else None, lst.step_dev.data_ptr(),
                                       lst.scalars.data_ptr(), st), 'sr_adamw_tick')
             run(0, lst.scalars.data_ptr(), table)
@@ -734,7 +737,20 @@ class AdamW(torch.optim.Optimizer):
         steps = [np.array([int(float(state.get(i, {}).get('step', 0))) for i in lst.members], dtype=np.int64) for lst in self._lists]
         if self.capturable and any(set(t.tolist()) - {0, int(t.max())} for t in steps):
             raise ValueError('AdamW.load_state_dict: capturable=True takes one step count')
-        for mine, hp in zip(self.param_groups, new):
+        rates = [(mine['lr'], float(hp['lr'])) for mine, hp in zip(self.param_groups, new)]
+        for (lr, value), hp in zip(rates, new):
+            if torch.is_tensor(lr) and lr.is_cuda and self.capturable:
+                if all(other == value for x, other in rates if x is lr):
+                    hp['lr'] = lr                      # captured steps read it where it is: the value goes there
+                elif any(x is lr for lst in self._lists for x in lst.rates):
+                    raise ValueError('AdamW.load_state_dict: groups with different rates, but a captured step reads one tensor for them')
+                else:
+                    hp['lr'] = torch.full_like(lr, value)
+            elif torch.is_tensor(hp['lr']) and hp['lr'].is_cuda and not self.capturable:
+                hp['lr'] = value                       # (every step would wait for it)
+        for mine, hp, (lr, value) in zip(self.param_groups, new, rates):
+            if hp['lr'] is lr and torch.is_tensor(lr):
+                lr.fill_(value)
             mine.update(hp)
 
         def part(name, i):

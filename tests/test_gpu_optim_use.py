@@ -243,3 +243,62 @@ def test_loading_takes_copies(T):
     other.param_groups[0]['note']['k'].append(2)
     other.param_groups[0]['betas'][1] = 0.5
     assert opt.param_groups[0]['note'] == {'k': [1]} and list(opt.param_groups[0]['betas']) == [0.9, 0.99]
+
+
+def test_loading_keeps_the_rate_on_the_device(T):
+    """A captured step reads the learning rate where it was: loading writes there."""
+    (p, opt), (q, ref) = _one(T, lr=torch.tensor(1e-2, device='cuda'), capturable=True), _one(T)
+    lr = opt.param_groups[0]['lr']
+    for x in (p, q):
+        x.grad = torch.linspace(-1, 1, 300, device='cuda')
+    opt.step()
+    ref.step()
+    saved = copy.deepcopy(opt.state_dict())
+    saved['param_groups'][0]['lr'] = torch.tensor(3e-3, device='cuda')
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]['lr'] is lr and float(lr) == float(np.float32(3e-3))
+    ref.param_groups[0]['lr'] = float(lr)
+    for k in range(3):
+        graph.replay()
+        ref.step()
+        torch.cuda.synchronize()
+        junk = torch.full((1000,), 7.0, device='cuda').sum()
+        assert torch.equal(p, q), k
+        if k == 1:      # and the dictionary's tensor is not the optimizer's
+            saved['param_groups'][0]['lr'].fill_(1.0)
+    assert bool(junk == 7000)
+    saved['param_groups'][0]['lr'] = 5e-4
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]['lr'] is lr and float(lr) == float(np.float32(5e-4))
+
+
+def test_loading_where_groups_share_the_rates_tensor(T):
+    def build(**kw):
+        ps = [nn.Parameter(torch.ones(30, device='cuda')) for _ in range(2)]
+        return ps, T.AdamW([{'params': [p]} for p in ps], lr=torch.tensor(1e-2, device='cuda'), **kw)
+    ps, opt = build(capturable=True)
+    lr = opt.param_groups[0]['lr']
+    assert opt.param_groups[1]['lr'] is lr
+    saved = opt.state_dict()
+    saved['param_groups'][0]['lr'], saved['param_groups'][1]['lr'] = 0.25, 0.25
+    opt.load_state_dict(saved)
+    assert [g['lr'] is lr for g in opt.param_groups] == [True, True] and float(lr) == 0.25
+    saved['param_groups'][1]['lr'] = 0.5
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    with pytest.raises(ValueError, match='captured'):
+        opt.load_state_dict(saved)
+    assert float(lr) == 0.25
+    _, free = build(capturable=True)
+    free.load_state_dict(saved)
+    assert [float(g['lr']) for g in free.param_groups] == [0.25, 0.5]
+    _, eager = build()
+    saved['param_groups'][1]['lr'] = torch.tensor(0.5, device='cuda')
+    eager.load_state_dict(saved)
+    assert eager.param_groups[1]['lr'] == 0.5 and not torch.is_tensor(eager.param_groups[1]['lr'])
