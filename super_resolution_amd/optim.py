@@ -404,7 +404,8 @@ class AdamW(torch.optim.Optimizer):
     state_dict() / load_state_dict() use torch.optim.AdamW's layout (float32 `exp_avg`, `exp_avg_sq`, `step`; plus `ema`), so a
     checkpoint moves between the two and between 32 and 8 bits; values that 8 bits hold come back as they were.
     capturable=True: the step count (and an lr given as a float32 GPU tensor) live on the device, for steps inside a captured
-    graph; every step then has to bring the same gradients.  Without it a step under capture raises."""
+    graph; every step then has to bring the same gradients.  Without it a step under capture raises.  After replays call
+    `replayed()`: what keeps packed weights under the parameters' version counters cannot see them otherwise."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, ema_decay=None, seed=0, capturable=False,
                  broadcast=True, group=None):
@@ -579,6 +580,11 @@ class AdamW(torch.optim.Optimizer):
             for lst, h, miss, table in zip(self._lists, hypers, missing, tables):
                 self._launch(lst, h, miss, table, factor, st)
         return loss
+
+    def replayed(self):
+        """To be called after a graph that holds a step was replayed, before the parameters are used outside it: a replay writes them
+        without moving their version counters, by which autograd's saved-tensor checks and the networks' packed weights tell."""
+        torch.autograd.graph.increment_version([p for p in self.params if not p.is_inference()])
 
     def _launch(self, lst, h, missing, table, factor, st):
         lib = L.lib()

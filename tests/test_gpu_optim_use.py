@@ -302,3 +302,37 @@ def test_loading_where_groups_share_the_rates_tensor(T):
     saved['param_groups'][1]['lr'] = torch.tensor(0.5, device='cuda')
     eager.load_state_dict(saved)
     assert eager.param_groups[1]['lr'] == 0.5 and not torch.is_tensor(eager.param_groups[1]['lr'])
+
+
+# ---- captured steps ------------------------------------------------------------------------------------------------------
+def test_replayed_steps_reach_what_is_cached(T):
+    """Networks keep packed weights under the parameters' version counters; replayed() moves them after replays of a captured step."""
+    import super_resolution_amd as sra
+    torch.manual_seed(0)
+    net = sra.SRVGGNetCompact(3, 3, 64, 2, 4).cuda()
+    x = torch.rand(1, 3, 16, 16, device='cuda')
+    opt = T.AdamW(net.parameters(), lr=1e-2, capturable=True)
+    for p in net.parameters():
+        p.grad = torch.randn_like(p)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+
+    def evaluate():
+        net.eval()
+        fresh = sra.SRVGGNetCompact(3, 3, 64, 2, 4).cuda().eval()
+        fresh.load_state_dict(net.state_dict())
+        with torch.no_grad():
+            return net(x), fresh(x)
+    a, b = evaluate()
+    assert torch.equal(a, b)
+    for _ in range(2):
+        graph.replay()
+        graph.replay()
+        before = [p._version for p in net.parameters()]
+        opt.replayed()
+        assert all(p._version > v for p, v in zip(net.parameters(), before))
+        c, d = evaluate()
+        assert torch.equal(c, d) and not torch.equal(a, c)
+        a = c
