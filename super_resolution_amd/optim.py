@@ -694,25 +694,28 @@ class AdamW(torch.optim.Optimizer):
         return [lst.steps] * lst.n if isinstance(lst.steps, int) else lst.steps.tolist()
 
     def state_dict(self):
-        """torch.optim.AdamW's layout: {'state': {i: {'step', 'exp_avg', 'exp_avg_sq'[, 'ema']}}, 'param_groups': [...]}."""
+        """torch.optim.AdamW's layout: {'state': {i: {'step', 'exp_avg', 'exp_avg_sq'[, 'ema']}}, 'param_groups': [...]}; with an average
+        also 'ema': {i: ...} for the parameters that took no step (they have no state there; their average moves all the same)."""
         steps = {}
         for lst in self._lists:
             steps.update(zip(lst.members, self._steps_of(lst)))
-        state = {}
-        if any(steps.values()):
-            m, v = self.moments()
-            ema = self.ema.clone() if self.ema is not None else None
-            for i in (i for i in range(len(self.params)) if steps[i]):
+        state, resting = {}, {}
+        ema = self.ema.clone() if self.ema is not None else None
+        m, v = self.moments() if any(steps.values()) else (None, None)
+        for i in range(len(self.params)):
+            if steps[i]:
                 state[i] = {'step': torch.tensor(float(steps[i])), 'exp_avg': self._shaped(m, i), 'exp_avg_sq': self._shaped(v, i)}
-                if ema is not None:     # (the average of a parameter that never moved is the parameter)
-                    state[i]['ema'] = self._shaped(ema, i)
+            if ema is not None and steps[i]:
+                state[i]['ema'] = self._shaped(ema, i)
+            elif ema is not None:
+                resting[i] = self._shaped(ema, i)
         groups, first = [], 0
         for g in self.param_groups:
             hp = {k: x for k, x in g.items() if k != 'params'}
             hp['params'] = list(range(first, first + len(g['params'])))
             first += len(g['params'])
             groups.append(hp)
-        return {'state': state, 'param_groups': groups}
+        return {'state': state, 'param_groups': groups, **({'ema': resting} if resting else {})}
 
     @torch.no_grad()
     def load_state_dict(self, sd):
@@ -727,9 +730,12 @@ class AdamW(torch.optim.Optimizer):
         place = {}
         for i, key in enumerate(k for g in groups for k in g['params']):
             place[key] = i
-        if any(k not in place for k in sd['state']):
+        resting = sd.get('ema') or {}
+        if any(k not in place for k in [*sd['state'], *resting]):
             raise ValueError('AdamW.load_state_dict: a state for a parameter that no group holds')
-        state = {place[k]: s for k, s in sd['state'].items()}
+        state = {place[k]: {'ema': x} for k, x in resting.items()}
+        for k, s in sd['state'].items():
+            state[place[k]] = {**state.get(place[k], {}), **s}
         for i, s in state.items():
             for name in ('exp_avg', 'exp_avg_sq', 'ema'):
                 if name in s and s[name].shape != self._layout[i][0]:

@@ -336,3 +336,42 @@ def test_replayed_steps_reach_what_is_cached(T):
         c, d = evaluate()
         assert torch.equal(c, d) and not torch.equal(a, c)
         a = c
+
+
+def test_the_average_of_parameters_without_a_step_is_saved(T):
+    """Weights loaded after construction: the average of a frozen layer is on its way from the old ones to them."""
+    def build():
+        ps = [nn.Parameter(torch.zeros(20, 30, device='cuda')), nn.Parameter(torch.zeros(50, device='cuda')), nn.Parameter(torch.zeros(6, 4, device='cuda'))]
+        ps[0].data = ps[0].data.t().contiguous().t()
+        return ps, T.AdamW(ps, ema_decay=0.9)
+    ps, opt = build()
+    with torch.no_grad():
+        for k, p in enumerate(ps):
+            p.copy_(torch.arange(p.numel(), device='cuda').view(p.shape) + 1.0 + k)
+    first = copy.deepcopy(opt.state_dict())              # before any step
+    for _ in range(3):
+        ps[1].grad = torch.ones(50, device='cuda')
+        opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    assert sorted(saved['state']) == [1] and bool((opt.ema_parameters()[0] < ps[0]).all())
+    for sd, want in ((saved, [e.clone() for e in opt.ema_parameters()]), (first, [torch.zeros_like(p) for p in ps])):
+        qs, other = build()
+        with torch.no_grad():
+            for p, q in zip(ps, qs):
+                q.copy_(p)
+        other.load_state_dict(sd)
+        for got, w in zip(other.ema_parameters(), want):
+            assert torch.equal(got, w)
+    bad = dict(saved, ema={0: torch.zeros(3)})
+    with pytest.raises(ValueError, match='ema'):
+        other.load_state_dict(bad)
+    with pytest.raises(ValueError, match='no group'):
+        other.load_state_dict(dict(saved, ema={9: torch.zeros(3)}))
+    # into torch's, and a dictionary without averages
+    topt = torch.optim.AdamW([nn.Parameter(p.detach().clone()) for p in ps])
+    topt.load_state_dict(saved)
+    other.load_state_dict({k: saved[k] for k in ('state', 'param_groups')})
+    assert torch.equal(other.ema_parameters()[0], qs[0]) and torch.equal(other.ema_parameters()[1], saved['state'][1]['ema'])
+    plain = T.AdamW([nn.Parameter(p.detach().clone()) for p in ps])
+    plain.load_state_dict(saved)
+    assert 'ema' not in plain.state_dict()
