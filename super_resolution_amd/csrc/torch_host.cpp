@@ -65,6 +65,27 @@ const at::Tensor* gradient_of(const c10::TensorImpl* t) {
     const auto* meta = static_cast<const torch::autograd::AutogradMeta*>(t->autograd_meta());
     return meta && meta->grad_.defined() ? &meta->grad_ : nullptr;
 }
+// takes a bump_version back: the tensor was not written after all
+void unbump_version(c10::TensorImpl* t) {
+    c10::VariableVersion v = t->version_counter();  // (shares the tensor's counter)
+    v.set_version((int64_t)v.current_version() - 1);
+}
+// the gradients of the first `count` tensors of a list whose versions srt_spans moved
+void unbump_gradients(PyObject* list, int of_params, Py_ssize_t count) {
+    for (Py_ssize_t i = 0; i < count; ++i) {
+        c10::TensorImpl* g = tensor_of(PyList_GET_ITEM(list, i)).unsafeGetTensorImpl();
+        const at::Tensor* grad = of_params ? gradient_of(g) : nullptr;
+        if (of_params && !grad) continue;
+        if (grad) g = grad->unsafeGetTensorImpl();
+        if (!g->is_inference()) unbump_version(g);
+    }
+}
+struct Walked {  // takes the bumps back when the walk ends early
+    PyObject* list;
+    int of_params;
+    Py_ssize_t count;
+    ~Walked() { unbump_gradients(list, of_params, count); }
+};
 // the same memory order: element i of one is element i of the other
 bool same_layout(const c10::TensorImpl* a, const c10::TensorImpl* b) {
     return (a->is_contiguous() && b->is_contiguous()) || (a->strides().equals(b->strides()) && a->is_non_overlapping_and_dense());
@@ -138,12 +159,24 @@ SRT_API int64_t srt_gradients(void* h, uint64_t* out, int64_t* odd, int64_t* nod
         return missing;
     });
 }
+// The step that srt_gradients prepared does not take place: the version counters go back.
+SRT_API int64_t srt_not_written(void* h) {
+    return guarded([&]() -> int64_t {
+        const Tracked& t = *(const Tracked*)h;
+        for (size_t i = 0; i < t.params.size(); ++i) {
+            c10::TensorImpl* p = t.params[i].unsafeGetTensorImpl();
+            if (t.was[i].counts && gradient_of(p)) unbump_version(p);
+        }
+        return 0;
+    });
+}
 
 // The gradients of a list of parameters (of_params) or of a list of gradients, as spans of consecutive values of at most
 // `longest` (0: by the total, see below); counts[0 / 1]: spans in float32 / bfloat16, counts[2]: tensors.  Returns 0, or
 //   1 + i: tensor i is neither float32 nor bfloat16, or not on GPU `device` (device < 0: that of the first, put into *device)
 //   -2 - i: gradient i has holes or repeats its elements
-// and SRT_FAILED.  Gradients that share memory fail: they would be scaled twice.
+// and SRT_FAILED.  Gradients that share memory fail: they would be scaled twice.  The version counters of the gradients move, as they
+// are about to be written, but not where the call fails.
 SRT_API int64_t srt_spans(PyObject* list, int of_params, int* device, int64_t* counts) {
     return guarded([&]() -> int64_t {
         TORCH_CHECK(PyList_Check(list), "not a list");
@@ -156,8 +189,10 @@ SRT_API int64_t srt_spans(PyObject* list, int of_params, int* device, int64_t* c
         bool ascending = true;
         const Py_ssize_t size = PyList_GET_SIZE(list);
         found[0].reserve(size);
+        Walked walked{list, of_params, 0};
         c10::DispatchKeySet usual;  // of the first gradient: those with the same keys are of the same kind
         for (Py_ssize_t i = 0; i < size; ++i) {
+            walked.count = i;
             c10::TensorImpl* g = tensor_of(PyList_GET_ITEM(list, i)).unsafeGetTensorImpl();
             if (of_params) {
                 const at::Tensor* grad = gradient_of(g);
@@ -170,10 +205,10 @@ SRT_API int64_t srt_spans(PyObject* list, int of_params, int* device, int64_t* c
                 if (*device < 0) *device = g->device().index();
                 if (!g->is_inference()) usual = g->key_set();
             }
-            if (g->key_set() == usual) g->bump_version();  // they are about to be written
             const int kind = g->dtype() == caffe2::TypeMeta::Make<float>() ? 0 : g->dtype() == caffe2::TypeMeta::Make<at::BFloat16>() ? 1 : -1;
             if (kind < 0 || g->device().index() != *device) return 1 + i;
             if (!g->is_contiguous() && !g->is_non_overlapping_and_dense()) return -2 - i;
+            if (g->key_set() == usual) g->bump_version();  // (not that of an inference tensor, which has none)
             const int64_t n = g->numel();
             if (!n) continue;
             const uint64_t at = (uint64_t)(uintptr_t)g->data();
@@ -182,6 +217,7 @@ SRT_API int64_t srt_spans(PyObject* list, int of_params, int* device, int64_t* c
             found[kind].push_back({at, n});
             total += n;
         }
+        walked.count = size;
         if (!ascending) {
             std::vector<std::pair<uint64_t, uint64_t>> all;
             for (int k = 0; k < 2; ++k)
@@ -194,6 +230,14 @@ SRT_API int64_t srt_spans(PyObject* list, int of_params, int* device, int64_t* c
         g_longest = longest;
         for (int k = 0; k < 2; ++k)
             for (const Span& s : found[k]) counts[k] += s.n <= longest ? 1 : (s.n + longest - 1) / longest;
+        walked.count = 0;
+        return 0;
+    });
+}
+// The gradients that srt_spans walked are not written: the version counters go back.
+SRT_API int64_t srt_spans_not_written(PyObject* list, int of_params) {
+    return guarded([&]() -> int64_t {
+        unbump_gradients(list, of_params, PyList_GET_SIZE(list));
         return 0;
     });
 }

@@ -35,6 +35,8 @@ def _host_lib():
         h.srt_untrack.restype, h.srt_untrack.argtypes = None, [C.c_void_p]
         h.srt_gradients.restype, h.srt_gradients.argtypes = C.c_int64, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
         h.srt_spans.restype, h.srt_spans.argtypes = C.c_int64, [C.py_object, C.c_int, C.c_void_p, C.c_void_p]
+        h.srt_not_written.restype, h.srt_not_written.argtypes = C.c_int64, [C.c_void_p]
+        h.srt_spans_not_written.restype, h.srt_spans_not_written.argtypes = C.c_int64, [C.py_object, C.c_int]
         h.srt_take_spans.restype, h.srt_take_spans.argtypes = None, [C.c_void_p]
         _host = h
     return _host
@@ -169,7 +171,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     host, lib = _host_lib(), L.lib()
     device, counts = C.c_int(-1), (C.c_int64 * 3)()
     rc = host.srt_spans(params, 1, C.byref(device), counts)
-    odd = []
+    odd, walked = [], (params, 1)
     if rc <= -2:   # gradients with holes: the norm reads dense copies, torch scales the originals
         grads = [(i, p.grad) for i, p in enumerate(params) if p.grad is not None]
         for i, g in grads:
@@ -178,8 +180,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         _check_separate(grads)
         odd = [g for _, g in grads if not _is_dense(g)]
         dense = [g if _is_dense(g) else g.detach().contiguous() for _, g in grads]      # (alive until the norm is launched)
-        device = C.c_int(-1)
-        rc = host.srt_spans(dense, 0, C.byref(device), counts)
+        device, walked = C.c_int(-1), (dense, 0)
+        rc = host.srt_spans(*walked, C.byref(device), counts)
     if rc == -1:
         _host_failed('clip_grad_norm_')
     if rc > 0:
@@ -189,18 +191,22 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     dev = torch.device('cuda', device.value)
     with _on(dev):
         st = _stream(dev)
-        n32, n16 = counts[0], counts[1]
-        stage = _Stage(16 * (n32 + n16))
-        host.srt_take_spans(stage.at)
-        on_host = int(n32 + n16 <= L.GRAD_SPANS_BY_VALUE)
-        spans = stage.at if on_host else stage.upload(dev, st)
-        first = spans if on_host else spans.data_ptr()
-        lists = (L.GradList * (1 + (n16 > 0 and n32 > 0)))()
-        for l, (at, n, code) in zip(lists, [x for x in ((first, n32, L.SR_F32), (first + 16 * n32, n16, L.SR_BF16)) if x[1]]):
-            l.spans, l.nspans, l.dtype, l.on_host = at, n, code, on_host
-        buf, norm = _norm(lists, max_norm, dev, st)
-        if error_if_nonfinite and not bool(torch.isfinite(norm)):
-            raise RuntimeError('clip_grad_norm_: the norm of the gradients is not finite')
+        try:
+            n32, n16 = counts[0], counts[1]
+            stage = _Stage(16 * (n32 + n16))
+            host.srt_take_spans(stage.at)
+            on_host = int(n32 + n16 <= L.GRAD_SPANS_BY_VALUE)
+            spans = stage.at if on_host else stage.upload(dev, st)
+            first = spans if on_host else spans.data_ptr()
+            lists = (L.GradList * (1 + (n16 > 0 and n32 > 0)))()
+            for l, (at, n, code) in zip(lists, [x for x in ((first, n32, L.SR_F32), (first + 16 * n32, n16, L.SR_BF16)) if x[1]]):
+                l.spans, l.nspans, l.dtype, l.on_host = at, n, code, on_host
+            buf, norm = _norm(lists, max_norm, dev, st)
+            if error_if_nonfinite and not bool(torch.isfinite(norm)):
+                raise RuntimeError('clip_grad_norm_: the norm of the gradients is not finite')
+        except BaseException:    # nothing was written
+            host.srt_spans_not_written(*walked)
+            raise
         for l in lists:
             if l.nspans:
                 L.check(lib.sr_grad_scale(l.dtype, l.nspans, l.spans, l.on_host, buf.data_ptr() + 4 * buf.numel() - 4, st), 'sr_grad_scale')
@@ -343,8 +349,9 @@ class _List:
         except Exception:   # interpreter shutdown
             pass
 
-    def gradients(self, keep):
-        """Fills self.ptrs; returns the number of tensors without a gradient.  keep: copies that must live until the launch."""
+    def gradients(self, keep, walked):
+        """Fills self.ptrs; returns the number of tensors without a gradient.  keep: copies that must live until the launch; walked: the
+        lists whose parameters' version counters have moved."""
         if self.n > L.ADAMW_BY_VALUE or self.ptrs is None:
             if self.n > L.ADAMW_BY_VALUE:
                 self.stage = _Stage(8 * self.n)
@@ -352,6 +359,7 @@ class _List:
         missing = _host_lib().srt_gradients(self.tracked, self.ptrs, self.odd, C.byref(self.nodd), C.byref(self.moved))
         if missing < 0:
             _host_failed('AdamW')
+        walked.append(self)
         for k in range(self.nodd.value):
             p = self.params[self.odd[k]]
             g = p.grad
@@ -561,22 +569,27 @@ class AdamW(torch.optim.Optimizer):
             capturing = torch.cuda.is_current_stream_capturing()
             if capturing and not self.capturable:
                 raise RuntimeError('AdamW: a step under graph capture needs capturable=True (the step count would stay what it is now)')
-            keep, hypers, missing = [], [], []
-            for lst in self._lists:   # everything that can fail comes before the first launch
-                hypers.append(self._hyper(self.param_groups[lst.group]))
-                missing.append(lst.gradients(keep))
-                if lst.moved.value:
-                    self._follow(lst, capturing)
-                if self.capturable and missing[-1] < lst.n:
-                    self._same_gradients(lst)
-            tables = [lst.table(dev, st) for lst in self._lists]
-            factor = None
-            if clip_grad_norm is not None:
-                lists = (L.GradList * len(self._lists))()
-                for l, lst, table in zip(lists, self._lists, tables):
-                    l.list, l.grads, l.on_host = lst.handle, table[0], table[1]
-                buf, self.grad_norm = _norm(lists, float(clip_grad_norm), dev, st)
-                factor = buf.data_ptr() + 4 * buf.numel() - 4
+            keep, walked, hypers, missing = [], [], [], []
+            try:
+                for lst in self._lists:   # everything that can fail comes before the first launch
+                    hypers.append(self._hyper(self.param_groups[lst.group]))
+                    missing.append(lst.gradients(keep, walked))
+                    if lst.moved.value:
+                        self._follow(lst, capturing)
+                    if self.capturable and missing[-1] < lst.n:
+                        self._same_gradients(lst)
+                tables = [lst.table(dev, st) for lst in self._lists]
+                factor = None
+                if clip_grad_norm is not None:
+                    lists = (L.GradList * len(self._lists))()
+                    for l, lst, table in zip(lists, self._lists, tables):
+                        l.list, l.grads, l.on_host = lst.handle, table[0], table[1]
+                    buf, self.grad_norm = _norm(lists, float(clip_grad_norm), dev, st)
+                    factor = buf.data_ptr() + 4 * buf.numel() - 4
+            except BaseException:    # nothing was written
+                for lst in walked:
+                    _host_lib().srt_not_written(lst.tracked)
+                raise
             for lst, h, miss, table in zip(self._lists, hypers, missing, tables):
                 self._launch(lst, h, miss, table, factor, st)
         return loss

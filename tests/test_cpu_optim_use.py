@@ -99,3 +99,29 @@ def test_shared_elements_against_a_list_of_all_bytes():
         else:
             optim._check_separate(list(enumerate(views)))
     assert min(found) > 100
+
+
+def test_a_refused_walk_leaves_version_counters(host):
+    ps = [nn.Parameter(torch.zeros(3)) for _ in range(4)]
+    for p in ps[1:]:
+        p.grad = torch.ones(3)
+    h, walk = _track(host, ps)
+    before = [p._version for p in ps]
+    walk()
+    assert [p._version - b for p, b in zip(ps, before)] == [0, 1, 1, 1]
+    assert host.srt_not_written(h) == 0
+    assert [p._version - b for p, b in zip(ps, before)] == [0, 0, 0, 0]
+    host.srt_untrack(h)
+    # a view and its base have one counter
+    base = torch.zeros(6)
+    ps = [nn.Parameter(t) for t in (base[:3].detach(), base[3:].detach())]
+    for p in ps:
+        p.grad = torch.ones(3)
+    h, walk = _track(host, ps)
+    before = [p._version for p in ps]
+    walk()
+    walk()
+    host.srt_not_written(h)
+    host.srt_not_written(h)
+    assert [p._version for p in ps] == before
+    host.srt_untrack(h)

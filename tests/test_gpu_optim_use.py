@@ -375,3 +375,57 @@ def test_the_average_of_parameters_without_a_step_is_saved(T):
     plain = T.AdamW([nn.Parameter(p.detach().clone()) for p in ps])
     plain.load_state_dict(saved)
     assert 'ema' not in plain.state_dict()
+
+
+# ---- refused calls -------------------------------------------------------------------------------------------------------
+def test_refused_calls_leave_version_counters(T):
+    """Autograd and the networks' caches take a moved counter for a write."""
+    def counters(ps):
+        return [(p._version, None if p.grad is None else p.grad._version) for p in ps]
+    whole = torch.ones(6, 16, device='cuda')
+    ps = [nn.Parameter(torch.ones(s, device='cuda')) for s in ((5,), (6, 8), (6, 8), (300,))]
+    ps[0].grad = torch.full((5,), float('inf'), device='cuda')
+    ps[3].grad = torch.ones(300, device='cuda')
+    before = counters(ps)
+    with pytest.raises(RuntimeError, match='finite'):
+        T.clip_grad_norm_(ps, 1.0, error_if_nonfinite=True)
+    assert counters(ps) == before
+    ps[1].grad = whole[:, ::2]
+    before = counters(ps)
+    with pytest.raises(RuntimeError, match='finite'):
+        T.clip_grad_norm_(ps, 1.0, error_if_nonfinite=True)
+    assert counters(ps) == before
+    ps[2].grad = ps[1].grad
+    before = counters(ps)
+    with pytest.raises(RuntimeError, match='share'):
+        T.clip_grad_norm_(ps, 1.0)
+    assert counters(ps) == before
+    ps[1].grad = ps[2].grad = torch.ones(6, 8, device='cuda')
+    before = counters(ps)
+    with pytest.raises(RuntimeError, match='share'):
+        T.clip_grad_norm_(ps, 1.0)
+    assert counters(ps) == before
+    ps[1].grad = None
+    half = nn.Parameter(torch.ones(3, device='cuda', dtype=torch.float16))
+    half.grad = torch.ones_like(half)
+    before = counters(ps + [half])
+    with pytest.raises(TypeError):
+        T.clip_grad_norm_(ps + [half], 1.0)
+    with pytest.raises(RuntimeError, match='not a tensor'):
+        T.clip_grad_norm_(ps + [3], 1.0)
+    assert counters(ps + [half]) == before
+    # steps: two groups, the second one refused
+    opt = T.AdamW([{'params': ps[:2]}, {'params': ps[2:]}], capturable=True)
+    opt.step()
+    ps[3].data = torch.ones(301, device='cuda')
+    ps[3].grad = None
+    before = counters(ps)
+    with pytest.raises(RuntimeError, match='rebuild'):
+        opt.step()
+    assert counters(ps) == before
+    ps[3].data = torch.ones(300, device='cuda')
+    ps[1].grad = torch.ones(6, 8, device='cuda')
+    before = counters(ps)
+    with pytest.raises(RuntimeError, match='same parameters'):
+        opt.step()
+    assert counters(ps) == before
