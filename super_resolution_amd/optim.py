@@ -464,8 +464,6 @@ class AdamW(torch.optim.Optimizer):
                     if members:
                         self._lists.append(_List(self, k, g['state_bits'], members))
                 first += len(g['params'])
-            if len(self._lists) > L.GRAD_MAX_LISTS:
-                raise ValueError('AdamW: at most %d parameter groups of one dtype' % L.GRAD_MAX_LISTS)
             for lst in self._lists:
                 lst.build(self)
         self.grad_norm = None   # of the last step with clip_grad_norm: a 0-d float32 tensor on the GPU
@@ -578,12 +576,16 @@ class AdamW(torch.optim.Optimizer):
                         self._follow(lst, capturing)
                     if self.capturable and missing[-1] < lst.n:
                         self._same_gradients(lst)
+                many = clip_grad_norm is not None and len(self._lists) > L.GRAD_MAX_LISTS
+                if many:
+                    lists = self._spans(keep, dev, st)
                 tables = [lst.table(dev, st) for lst in self._lists]
                 factor = None
                 if clip_grad_norm is not None:
-                    lists = (L.GradList * len(self._lists))()
-                    for l, lst, table in zip(lists, self._lists, tables):
-                        l.list, l.grads, l.on_host = lst.handle, table[0], table[1]
+                    if not many:
+                        lists = (L.GradList * len(self._lists))()
+                        for l, lst, table in zip(lists, self._lists, tables):
+                            l.list, l.grads, l.on_host = lst.handle, table[0], table[1]
                     buf, self.grad_norm = _norm(lists, float(clip_grad_norm), dev, st)
                     factor = buf.data_ptr() + 4 * buf.numel() - 4
             except BaseException:    # nothing was written
@@ -593,6 +595,28 @@ class AdamW(torch.optim.Optimizer):
             for lst, h, miss, table in zip(self._lists, hypers, missing, tables):
                 self._launch(lst, h, miss, table, factor, st)
         return loss
+
+    def _spans(self, keep, dev, st):
+        """The gradients of more lists than one norm takes, as one list of spans per dtype."""
+        lists = (L.GradList * 2)()
+        for l, dt in zip(lists, (torch.float32, torch.bfloat16)):
+            l.dtype = L.dtype_code(dt)
+            part = [lst for lst in self._lists if lst.dtype == dt]
+            if not part:
+                continue
+            at, n = np.concatenate([np.frombuffer(lst.ptrs, dtype=np.uint64) for lst in part]), np.concatenate([lst.sizes for lst in part])
+            at, n = at[(at != 0) & (n > 0)], n[(at != 0) & (n > 0)]
+            longest = max(4096, -(-int(n.sum()) // 8192 // 1024) * 1024)     # as clip_grad_norm_ shares long tensors out
+            pieces = -(-n // longest)
+            first = (np.arange(int(pieces.sum())) - np.repeat(np.cumsum(pieces) - pieces, pieces)) * longest
+            spans = np.stack([np.repeat(at.astype(np.int64), pieces) + first * dt.itemsize, np.minimum(np.repeat(n, pieces) - first, longest)], axis=1)
+            if len(spans):
+                stage = _Stage(spans.nbytes)
+                C.memmove(stage.at, np.ascontiguousarray(spans).ctypes.data, spans.nbytes)
+                table = stage.upload(dev, st)
+                keep.append(table)
+                l.spans, l.nspans = table.data_ptr(), len(spans)
+        return lists
 
     def replayed(self):
         """To be called after a graph that holds a step was replayed, before the parameters are used outside it: a replay writes them

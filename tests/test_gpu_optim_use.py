@@ -429,3 +429,32 @@ def test_refused_calls_leave_version_counters(T):
     with pytest.raises(RuntimeError, match='same parameters'):
         opt.step()
     assert counters(ps) == before
+
+
+@pytest.mark.parametrize('bf16', [False, True])
+def test_more_groups_than_a_norm_takes_lists(T, bf16):
+    """Layer-wise rates: 150 groups, with the norm of the whole, tensors without a gradient and empty ones among them."""
+    rng = np.random.default_rng(9)
+    sizes = [1 + (617 * i) % 3001 for i in range(150)]
+    sizes[3], sizes[7], sizes[149] = 0, 70001, 5
+    arrays = [rng.standard_normal(n).astype(np.float32) for n in sizes]
+    dts = [torch.bfloat16 if bf16 and i % 3 == 0 else torch.float32 for i in range(150)]
+    arrays = [torch.from_numpy(a).to(d).float().numpy() for a, d in zip(arrays, dts)]
+    params = [nn.Parameter(f32(a).to(d)) for a, d in zip(arrays, dts)]
+    starts = np.cumsum([0] + sizes)
+    opt = T.AdamW([{'params': [p], 'lr': 1e-3 * (1 + i % 7)} for i, p in enumerate(params)], seed=3, **HP)
+    refs = [R.Tensors([a], dict(HP, lr=1e-3 * (1 + i % 7)), 32, d == torch.bfloat16, 3, int(at)) for i, (a, d, at) in enumerate(zip(arrays, dts, starts))]
+    for clip in (None, 0.5, 1e9):
+        gs = [torch.from_numpy(rng.standard_normal(n).astype(np.float32)).to(d).float().numpy() for n, d in zip(sizes, dts)]
+        for i in (11, 64, 149):
+            gs[i] = None
+        norm = np.sqrt(sum(float(np.sum(g.astype(np.float64) ** 2)) for g in gs if g is not None))
+        factor = 1.0 if clip is None else min(1.0, clip / (norm + 1e-6))
+        for p, g, d, r in zip(params, gs, dts, refs):
+            p.grad = None if g is None else f32(g).to(d)
+            r.step([None if g is None else g * np.float32(factor)])
+        opt.step(clip_grad_norm=clip)
+        if clip is not None:
+            assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm
+    for i, (p, r) in enumerate(zip(params, refs)):
+        same(p, r.p[0], 'p[%d]' % i)
