@@ -299,7 +299,9 @@ class _List:
         self.ptrs, self.stage = None, _Stage(8 * self.n) if self.n <= L.ADAMW_BY_VALUE else None
         self.odd = (C.c_int64 * self.n)()
         self.nodd, self.moved = C.c_int64(), C.c_int64()
-        self.seen = self.step_dev = self.scalars = None
+        self.step_dev = self.scalars = None
+        self.loaded = np.zeros(self.n, dtype=np.int64)      # capturable: step counts that a checkpoint brought, and the tensors that
+        self.seen = self.captured = None                    # count on the device since then (of the last step, of the last captured one)
         self.rates = []             # learning rates on the device that captured steps read
         if opt.capturable:          # fixed memory: captured graphs point to it
             self.step_dev = torch.zeros((), dtype=torch.int64, device=opt.device)
@@ -567,7 +569,7 @@ class AdamW(torch.optim.Optimizer):
             capturing = torch.cuda.is_current_stream_capturing()
             if capturing and not self.capturable:
                 raise RuntimeError('AdamW: a step under graph capture needs capturable=True (the step count would stay what it is now)')
-            keep, walked, hypers, missing = [], [], [], []
+            keep, walked, hypers, missing, seen = [], [], [], [], []
             try:
                 for lst in self._lists:   # everything that can fail comes before the first launch
                     hypers.append(self._hyper(self.param_groups[lst.group]))
@@ -575,7 +577,7 @@ class AdamW(torch.optim.Optimizer):
                     if lst.moved.value:
                         self._follow(lst, capturing)
                     if self.capturable and missing[-1] < lst.n:
-                        self._same_gradients(lst)
+                        seen.append((lst, self._same_gradients(lst)))
                 many = clip_grad_norm is not None and len(self._lists) > L.GRAD_MAX_LISTS
                 if many:
                     lists = self._spans(keep, dev, st)
@@ -592,6 +594,10 @@ class AdamW(torch.optim.Optimizer):
                 for lst in walked:
                     _host_lib().srt_not_written(lst.tracked)
                 raise
+            for lst, have in seen:
+                lst.seen = have
+                if capturing:
+                    lst.captured = have
             for lst, h, miss, table in zip(self._lists, hypers, missing, tables):
                 self._launch(lst, h, miss, table, factor, st)
         return loss
@@ -716,9 +722,13 @@ class AdamW(torch.optim.Optimizer):
         """One step count on the device serves all tensors of a list."""
         have = np.frombuffer(lst.ptrs, dtype=np.uint64) != 0
         if lst.seen is None:
-            lst.seen = have.copy()
+            other = lst.loaded[have] != lst.loaded.max()
+            if other.any():
+                raise RuntimeError('AdamW(capturable=True): one step count serves all tensors, but of those with a gradient %d have not the %d steps of the '
+                                   'checkpoint' % (other.sum(), lst.loaded.max()))
         elif not np.array_equal(lst.seen, have):
             raise RuntimeError('AdamW(capturable=True): a step must bring gradients for the same parameters as the one before')
+        return have
 
     # ---- checkpoints ---------------------------------------------------------------------------------------------------
     # group keys that belong to this optimizer's layout, or to the implementation that wrote the dictionary
@@ -726,8 +736,10 @@ class AdamW(torch.optim.Optimizer):
 
     def _steps_of(self, lst):
         if self.capturable:
-            t = int(lst.step_dev.item())
-            return [t if lst.seen is None or lst.seen[i] else 0 for i in range(lst.n)]
+            counting = lst.seen if lst.seen is not None else lst.captured
+            if counting is None:
+                return lst.loaded.tolist()
+            return np.where(counting & (lst.loaded == lst.loaded.max()), int(lst.step_dev.item()), lst.loaded).tolist()
         return [lst.steps] * lst.n if isinstance(lst.steps, int) else lst.steps.tolist()
 
     def state_dict(self):
@@ -822,7 +834,7 @@ class AdamW(torch.optim.Optimizer):
             for lst, t in zip(self._lists, steps):
                 if self.capturable:
                     lst.step_dev.fill_(int(t.max()))
-                    lst.seen = None
+                    lst.loaded, lst.seen = t, None
                 else:
                     lst.steps = int(t[0]) if (t == t[0]).all() else t
             if self.ema is not None and self.numel:

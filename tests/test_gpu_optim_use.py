@@ -458,3 +458,55 @@ def test_more_groups_than_a_norm_takes_lists(T, bf16):
             assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm
     for i, (p, r) in enumerate(zip(params, refs)):
         same(p, r.p[0], 'p[%d]' % i)
+
+
+def test_capturable_loads_parameters_without_a_step(T):
+    """One count on the device serves the parameters that have one: the others keep theirs, and may not join later."""
+    def build(n=3, **kw):
+        ps = [nn.Parameter(torch.ones(40 + k, device='cuda')) for k in range(n)]
+        return ps, T.AdamW(ps, **dict(HP, **kw))
+    ps, opt = build()
+    for p in ps[:2]:
+        p.grad = torch.ones_like(p)
+    for _ in range(4):
+        opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    qs, cap = build(capturable=True)
+    with torch.no_grad():
+        for p, q in zip(ps, qs):
+            q.copy_(p)
+    cap.load_state_dict(saved)
+    assert sorted(cap.state_dict()['state']) == [0, 1]
+    for q in qs:
+        q.grad = torch.ones_like(q)
+    with pytest.raises(RuntimeError, match='count'):
+        cap.step()
+    assert torch.equal(qs[0], ps[0])
+    qs[2].grad = None
+    opt.step()
+    cap.step()
+    assert torch.equal(qs[0], ps[0]) and torch.equal(qs[1], ps[1])
+    assert {i: int(s['step']) for i, s in cap.state_dict()['state'].items()} == {0: 5, 1: 5}
+    # a part of what was loaded goes on: the rest keeps its moments and its count
+    rs, part = build(capturable=True)
+    part.load_state_dict(saved)
+    rs[0].grad = torch.ones_like(rs[0])
+    part.step()
+    s = part.state_dict()['state']
+    assert {i: int(x['step']) for i, x in s.items()} == {0: 5, 1: 4} and torch.equal(s[1]['exp_avg'], saved['state'][1]['exp_avg'])
+
+
+def test_replays_after_loading_are_counted(T):
+    p, opt = _one(T, capturable=True)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(2):
+        opt.load_state_dict(saved)
+        assert int(opt.state_dict()['state'][0]['step']) == 1
+        graph.replay()
+        graph.replay()
+        assert int(opt.state_dict()['state'][0]['step']) == 3
