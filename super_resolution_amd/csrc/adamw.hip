@@ -271,7 +271,7 @@ __device__ __forceinline__ uint16_t round_bf16(float x, uint32_t h) {
 // instructions, which is what bounds the step with 8-bit moments.  rsq / rcp are good to one ulp; one correction by the exact
 // residual rounds the root correctly (checked for all 2^24 significands) and the reciprocal (all 2^23), and with a correctly
 // rounded reciprocal the same correction rounds the quotient correctly (Markstein's theorem).  The ranges below keep every
-// residual exact: 0 <= x < 2^124, no subnormals but 0; |a| 0 or in [2^-85, 2^84], b in [2^-40, 2^41].
+// residual exact: 0 <= x < 2^124, no subnormals but 0; |a| 0 or in [2^-85, 2^84], b in [2^-40, 2^57].
 __device__ __forceinline__ float root(float x) {
     const float y = __builtin_amdgcn_rsqf(fmaxf(x, 0x1p-100f));
     const float r = x * y;
@@ -296,9 +296,13 @@ __device__ __forceinline__ void weights4(const Scalars& s, float (&p)[4], const 
 #pragma unroll
     for (int j = 0; j < 4; ++j) p[j] = p[j] * s.decay - (m[j] / (sqrtf(v[j]) * s.rbc2 + s.eps)) * s.step_size;
 }
-// The same for v < 2^60, |m| < 2^20 and eps >= 2^-40, as a block's exponents tell.  v and m are raised by 2^64 first (which keeps
-// subnormals in range) and the constants that follow take it back: exact, so the results are the same bits unless the quotient
-// itself is subnormal, where this one does not round it and the update is below 2^-126.
+// The same for v < 2^60 and |m| < 2^20, as a block's exponents tell, and for constants in_range().  v and m are raised by 2^64 first
+// (which keeps subnormals in range) and the constants that follow take it back: exact, so the results are the same bits unless the
+// quotient itself is subnormal, where this one does not round it and the update is below 2^-126.
+__device__ __forceinline__ bool in_range(const Scalars& s) {
+    // the divisor between 2^-40 and 2^57 (1 - b2 is 2^-53 at least), and step_size * 2^-64 normal
+    return s.eps >= 0x1p-40f && s.eps <= 0x1p40f && s.step_size >= 0x1p-60f;
+}
 __device__ __forceinline__ void weights4_in_range(const Scalars& s, float (&p)[4], const float (&m)[4], const float (&v)[4]) {
     const float rbc2 = s.rbc2 * 0x1p-32f, step_size = s.step_size * 0x1p-64f;
 #pragma unroll
@@ -361,7 +365,7 @@ __device__ __forceinline__ void step_piece(const Rec& r, const void* grad, const
             em |= a << 8 * k;
             ev |= b << 8 * k;
         }
-        if (BITS == 8 && a < 127 + 20 && b < 127 + 60 && s.eps >= 0x1p-40f)
+        if (BITS == 8 && a < 127 + 20 && b < 127 + 60 && in_range(s))
             weights4_in_range(s, p[k], m[k], v[k]);
         else
             weights4(s, p[k], m[k], v[k]);

@@ -510,3 +510,20 @@ def test_replays_after_loading_are_counted(T):
         graph.replay()
         graph.replay()
         assert int(opt.state_dict()['state'][0]['step']) == 3
+
+
+# ---- 8-bit moments at the ends of the range ------------------------------------------------------------------------------
+@pytest.mark.parametrize('lr,eps', [(1e-18, 1e-8), (1e-19, 1e-8), (1e-22, 1e-8), (1e-27, 1e-8), (1e-36, 1e-8), (1e-2, 1e12), (1e30, 1e35), (1e30, 1e38)])
+def test_rates_and_eps_at_the_ends_bit_for_bit(T, lr, eps):
+    """Weights of zero show every bit of the update, also where the rate, scaled inside the kernel, would leave the normal range."""
+    hp = dict(HP, lr=lr, eps=eps, weight_decay=0.0)
+    rng = np.random.default_rng(4)
+    p = nn.Parameter(torch.zeros(2000, device='cuda'))
+    opt = T.AdamW([p], state_bits=8, **hp)
+    ref = R.Tensors([np.zeros(2000, np.float32)], hp, 8)
+    for step in range(3):
+        g = rng.standard_normal(2000).astype(np.float32)
+        p.grad = f32(g)
+        opt.step()
+        ref.step([g])
+        same(p, ref.p[0], 'p, step %d' % step)
