@@ -80,12 +80,6 @@ void unbump_gradients(PyObject* list, int of_params, Py_ssize_t count) {
         if (!g->is_inference()) unbump_version(g);
     }
 }
-struct Walked {  // takes the bumps back when the walk ends early
-    PyObject* list;
-    int of_params;
-    Py_ssize_t count;
-    ~Walked() { unbump_gradients(list, of_params, count); }
-};
 // the same memory order: element i of one is element i of the other
 bool same_layout(const c10::TensorImpl* a, const c10::TensorImpl* b) {
     return (a->is_contiguous() && b->is_contiguous()) || (a->strides().equals(b->strides()) && a->is_non_overlapping_and_dense());
@@ -136,12 +130,14 @@ SRT_API int64_t srt_gradients(void* h, uint64_t* out, int64_t* odd, int64_t* nod
         for (size_t i = 0; i < n; ++i) {
             c10::TensorImpl* p = t.params[i].unsafeGetTensorImpl();
             const Tracked::Was& was = t.was[i];
-            // (another device: another storage)
             const bool contiguous = p->is_contiguous();
-            if (p->unsafe_storage().unsafeGetStorageImpl() != was.storage || p->data() != was.data || p->numel() != was.numel || p->dtype() != was.dtype ||
-                contiguous != was.contiguous || !(contiguous || p->strides().equals(t.strides[strided])))
-                ++*moved;
-            strided += !was.contiguous;
+            bool stayed = p->unsafe_storage().unsafeGetStorageImpl() == was.storage && p->data() == was.data && p->numel() == was.numel &&
+                          p->dtype() == was.dtype;  // (another device: another storage)
+            if (!(contiguous && was.contiguous)) {
+                stayed = stayed && contiguous == was.contiguous && p->strides().equals(t.strides[strided]);
+                strided += !was.contiguous;
+            }
+            *moved += !stayed;
             const at::Tensor* grad = gradient_of(p);
             out[i] = 0;
             if (!grad) {
@@ -189,48 +185,54 @@ SRT_API int64_t srt_spans(PyObject* list, int of_params, int* device, int64_t* c
         bool ascending = true;
         const Py_ssize_t size = PyList_GET_SIZE(list);
         found[0].reserve(size);
-        Walked walked{list, of_params, 0};
         c10::DispatchKeySet usual;  // of the first gradient: those with the same keys are of the same kind
-        for (Py_ssize_t i = 0; i < size; ++i) {
-            walked.count = i;
-            c10::TensorImpl* g = tensor_of(PyList_GET_ITEM(list, i)).unsafeGetTensorImpl();
-            if (of_params) {
-                const at::Tensor* grad = gradient_of(g);
-                if (!grad) continue;
-                g = grad->unsafeGetTensorImpl();
+        Py_ssize_t i = 0;
+        const auto refuse = [&](int64_t code) {
+            unbump_gradients(list, of_params, i);
+            return code;
+        };
+        try {
+            for (; i < size; ++i) {
+                c10::TensorImpl* g = tensor_of(PyList_GET_ITEM(list, i)).unsafeGetTensorImpl();
+                if (of_params) {
+                    const at::Tensor* grad = gradient_of(g);
+                    if (!grad) continue;
+                    g = grad->unsafeGetTensorImpl();
+                }
+                ++counts[2];
+                if (!(g->key_set() == usual)) {
+                    if (g->layout() != at::kStrided || !g->device().is_cuda()) return refuse(1 + i);
+                    if (*device < 0) *device = g->device().index();
+                    if (!g->is_inference()) usual = g->key_set();
+                }
+                const int kind = g->dtype() == caffe2::TypeMeta::Make<float>() ? 0 : g->dtype() == caffe2::TypeMeta::Make<at::BFloat16>() ? 1 : -1;
+                if (kind < 0 || g->device().index() != *device) return refuse(1 + i);
+                if (!g->is_contiguous() && !g->is_non_overlapping_and_dense()) return refuse(-2 - i);
+                if (g->key_set() == usual) g->bump_version();  // (not that of an inference tensor, which has none)
+                const int64_t n = g->numel();
+                if (!n) continue;
+                const uint64_t at = (uint64_t)(uintptr_t)g->data();
+                ascending &= at >= last;
+                last = at + (uint64_t)n * (kind ? 2 : 4);
+                found[kind].push_back({at, n});
+                total += n;
             }
-            ++counts[2];
-            if (!(g->key_set() == usual)) {
-                if (g->layout() != at::kStrided || !g->device().is_cuda()) return 1 + i;
-                if (*device < 0) *device = g->device().index();
-                if (!g->is_inference()) usual = g->key_set();
+            if (!ascending) {
+                std::vector<std::pair<uint64_t, uint64_t>> all;
+                for (int k = 0; k < 2; ++k)
+                    for (const Span& s : found[k]) all.emplace_back(s.g, s.g + (uint64_t)s.n * (k ? 2 : 4));
+                std::sort(all.begin(), all.end());
+                for (size_t i = 1; i < all.size(); ++i) TORCH_CHECK(all[i].first >= all[i - 1].second, "two gradients share memory");
             }
-            const int kind = g->dtype() == caffe2::TypeMeta::Make<float>() ? 0 : g->dtype() == caffe2::TypeMeta::Make<at::BFloat16>() ? 1 : -1;
-            if (kind < 0 || g->device().index() != *device) return 1 + i;
-            if (!g->is_contiguous() && !g->is_non_overlapping_and_dense()) return -2 - i;
-            if (g->key_set() == usual) g->bump_version();  // (not that of an inference tensor, which has none)
-            const int64_t n = g->numel();
-            if (!n) continue;
-            const uint64_t at = (uint64_t)(uintptr_t)g->data();
-            ascending &= at >= last;
-            last = at + (uint64_t)n * (kind ? 2 : 4);
-            found[kind].push_back({at, n});
-            total += n;
-        }
-        walked.count = size;
-        if (!ascending) {
-            std::vector<std::pair<uint64_t, uint64_t>> all;
-            for (int k = 0; k < 2; ++k)
-                for (const Span& s : found[k]) all.emplace_back(s.g, s.g + (uint64_t)s.n * (k ? 2 : 4));
-            std::sort(all.begin(), all.end());
-            for (size_t i = 1; i < all.size(); ++i) TORCH_CHECK(all[i].first >= all[i - 1].second, "two gradients share memory");
+        } catch (...) {
+            refuse(0);
+            throw;
         }
         // a wave takes a span at a time and 8192 waves run at once: equal shares of long tensors, none below 4096 values
         const int64_t longest = std::max<int64_t>(4096, (total / 8192 + 1023) / 1024 * 1024);
         g_longest = longest;
         for (int k = 0; k < 2; ++k)
             for (const Span& s : found[k]) counts[k] += s.n <= longest ? 1 : (s.n + longest - 1) / longest;
-        walked.count = 0;
         return 0;
     });
 }

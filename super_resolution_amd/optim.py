@@ -437,8 +437,11 @@ class AdamW(torch.optim.Optimizer):
             if not _is_dense(p):
                 raise ValueError('AdamW: a parameter with holes or repeated elements')
         self._check_overlap()
-        # shape, strides and order of the elements that moments and average are kept in
-        self._layout = [self._layout_now(p) for p in self.params]
+        # the shapes, and strides where not contiguous, that moments and average are kept in
+        self._shape, self._stride = [tuple(p.shape) for p in self.params], {}
+        for i, p in enumerate(self.params):
+            if not p.is_contiguous():
+                self._stride[i] = p.stride()
         # places: element number among all parameters; offset among the tensors of the same kind of moments; first block
         size = np.array([p.numel() for p in self.params], dtype=np.int64)
         bits = np.repeat([g['state_bits'] for g in self.param_groups], [len(g['params']) for g in self.param_groups])
@@ -513,14 +516,10 @@ class AdamW(torch.optim.Optimizer):
                 return torch._utils._flatten_dense_tensors(tensors)    # one C++ call for thousands of tensors
             return torch.cat([t.as_strided((t.numel(),), (1,)).float() for t in tensors])
 
-    @staticmethod
-    def _layout_now(p):
-        return p.shape, p.stride(), p.is_contiguous()
-
-    def _shaped(self, flat, i):
-        """Tensor i's part of a flat array, with its elements at the parameter's indices."""
-        at, (shape, stride, _) = int(self._index[i]), self._layout[i]
-        return flat[at:at + shape.numel()].as_strided(shape, stride)
+    def _shaped(self, flat):
+        """The parameters' parts of a flat array, with the elements at the parameters' indices."""
+        parts = flat.split([p.numel() for p in self.params])
+        return [x.as_strided(shape, self._stride[i]) if i in self._stride else x.view(shape) for i, (x, shape) in enumerate(zip(parts, self._shape))]
 
     @property
     def exp_avg(self):
@@ -550,7 +549,7 @@ class AdamW(torch.optim.Optimizer):
         """The average of the weights, one float32 view of `ema` per parameter."""
         if self.ema is None:
             raise RuntimeError('AdamW: built without ema_decay')
-        return [self._shaped(self.ema, i) for i in range(len(self.params))]
+        return self._shaped(self.ema)
 
     # ---- step ----------------------------------------------------------------------------------------------------------
     def step(self, closure=None, group=None, average=True, clip_grad_norm=None):
@@ -669,10 +668,9 @@ class AdamW(torch.optim.Optimizer):
         """Parameters lie elsewhere (`.data =`): same dtype, device and size are followed, anything else is refused."""
         turned = []
         for i, p in zip(lst.members, lst.params):
-            shape, stride, contiguous = self._layout[i]
-            if p.device != self.device or p.dtype != lst.dtype or p.shape != shape or not _is_dense(p):
+            if p.device != self.device or p.dtype != lst.dtype or p.shape != self._shape[i] or not _is_dense(p):
                 raise RuntimeError('AdamW: a parameter was moved, cast or resized after the optimizer was built -- rebuild the optimizer')
-            if p.stride() != stride and not (contiguous and p.is_contiguous()):
+            if (None if p.is_contiguous() else p.stride()) != self._stride.get(i):
                 turned.append(i)
         if capturing:
             raise RuntimeError('AdamW: a parameter was re-pointed; run one step outside the capture first')
@@ -686,11 +684,12 @@ class AdamW(torch.optim.Optimizer):
         """The memory order of parameter i has changed (channels_last and back): its moments and its average follow, so that every
         element keeps its own.  Blocks of 8-bit moments then hold other elements, and these are rounded once more."""
         p, n = self.params[i], self.params[i].numel()
-        shape, stride, _ = self._layout[i]
+        shape, stride = self._shape[i], self._stride.get(i)
         index, at, block = int(self._index[i]), int(self._at[i]), int(self._block[i])
 
         def turn(x):
-            x.as_strided(p.shape, p.stride()).copy_(x.clone().as_strided(shape, stride))
+            old = x.clone()
+            x.as_strided(p.shape, p.stride()).copy_(old.as_strided(shape, stride) if stride else old.view(shape))
         if bits == 32:
             turn(self._m32[at:at + n])
             turn(self._v32[at:at + n])
@@ -710,7 +709,10 @@ class AdamW(torch.optim.Optimizer):
                 lib.sr_adamw_destroy(h)
         if self.ema is not None:
             turn(self.ema[index:index + n])
-        self._layout[i] = self._layout_now(p)
+        if p.is_contiguous():
+            del self._stride[i]
+        else:
+            self._stride[i] = p.stride()
 
     def _check_overlap(self):
         spans = np.array([(p.data_ptr(), p.numel() * p.element_size()) for p in self.params if p.numel()], dtype=np.int64).reshape(-1, 2)
@@ -749,15 +751,16 @@ class AdamW(torch.optim.Optimizer):
         for lst in self._lists:
             steps.update(zip(lst.members, self._steps_of(lst)))
         state, resting = {}, {}
-        ema = self.ema.clone() if self.ema is not None else None
-        m, v = self.moments() if any(steps.values()) else (None, None)
-        for i in range(len(self.params)):
-            if steps[i]:
-                state[i] = {'step': torch.tensor(float(steps[i])), 'exp_avg': self._shaped(m, i), 'exp_avg_sq': self._shaped(v, i)}
-            if ema is not None and steps[i]:
-                state[i]['ema'] = self._shaped(ema, i)
-            elif ema is not None:
-                resting[i] = self._shaped(ema, i)
+        if any(steps.values()):
+            m, v = (self._shaped(x) for x in self.moments())
+            for i in (i for i in range(len(self.params)) if steps[i]):
+                state[i] = {'step': torch.tensor(float(steps[i])), 'exp_avg': m[i], 'exp_avg_sq': v[i]}
+        if self.ema is not None:
+            for i, x in enumerate(self._shaped(self.ema.clone())):
+                if steps[i]:
+                    state[i]['ema'] = x
+                else:
+                    resting[i] = x
         groups, first = [], 0
         for g in self.param_groups:
             hp = {k: x for k, x in g.items() if k != 'params'}
@@ -787,9 +790,8 @@ class AdamW(torch.optim.Optimizer):
             state[place[k]] = {**state.get(place[k], {}), **s}
         for i, s in state.items():
             for name in ('exp_avg', 'exp_avg_sq', 'ema'):
-                if name in s and s[name].shape != self._layout[i][0]:
-                    raise ValueError('AdamW.load_state_dict: parameter %d has shape %s, its %s %s'
-                                     % (i, tuple(self._layout[i][0]), name, tuple(s[name].shape)))
+                if name in s and s[name].shape != self._shape[i]:
+                    raise ValueError('AdamW.load_state_dict: parameter %d has shape %s, its %s %s' % (i, self._shape[i], name, tuple(s[name].shape)))
         # the rates, and what schedulers keep beside them
         new = [{**{k: mine[k] for k in ('lr', 'betas', 'eps', 'weight_decay')}, **{k: copy.deepcopy(x) for k, x in g.items() if k not in self._NOT_LOADED}}
                for g, mine in zip(groups, self.param_groups)]
@@ -815,13 +817,15 @@ class AdamW(torch.optim.Optimizer):
             mine.update(hp)
 
         def part(name, i):
-            shape, stride, _ = self._layout[i]
-            x = state.get(i, {}).get(name, self.params[i] if name == 'ema' else None)
+            p, stride = self.params[i], self._stride.get(i)
+            x = state.get(i, {}).get(name, p if name == 'ema' else None)
             if x is None:
-                return torch.zeros(shape.numel(), dtype=torch.float32, device=self.device)
+                return torch.zeros(p.numel(), dtype=torch.float32, device=self.device)
             if x.dtype != torch.float32 or x.device != self.device:
                 x = x.to(self.device, torch.float32)
-            return x if x.stride() == stride else torch.empty_strided(shape, stride, dtype=torch.float32, device=self.device).copy_(x)
+            if stride is None:
+                return x.contiguous()
+            return x if x.stride() == stride else torch.empty_strided(self._shape[i], stride, dtype=torch.float32, device=self.device).copy_(x)
 
         def flat(name):
             return self._cat([part(name, i) for i in range(len(self.params))])
