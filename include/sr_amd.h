@@ -358,7 +358,8 @@ int sr_fdconv_weightgen_backward(int B, const float* pooled, int pooled_ld, cons
  *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) (1 - b2^t)^-1/2 + eps);  ema = d ema + (1-d) p
  * in float32, one rounding per operation.  bits = 8: SR_ADAMW_BLOCK consecutive values of a tensor share an exponent byte; m is
  * held as sign + 4 exponent + 3 mantissa bits, v as 5 + 3, rounded stochastically by a hash of (seed, step, element number), as
- * bfloat16 parameters are.  v > 0 is never rounded to 0.  A block in which a moment is not finite decodes to NaN as a whole. */
+ * bfloat16 parameters are.  v > 0 is never rounded to 0.  A block in which a moment is not finite, or above 1.875 * 2^127 in
+ * magnitude, decodes to NaN as a whole. */
 #define SR_ADAMW_BLOCK 256
 #define SR_ADAMW_SCALARS_BYTES 64
 #define SR_ADAMW_SKIP ((uintptr_t)1) /* in a gradient table: leave this tensor alone (NULL: no gradient, only its average moves) */

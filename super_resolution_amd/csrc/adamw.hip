@@ -16,8 +16,8 @@
 // to nearest it would never move; rounded so, its mean is right.  v' > 0 does not round to 0 (m' / (sqrt(0) + eps) would be a
 // step of 1 / eps).  bfloat16 weights are rounded the same way for the same reason.  The random bits are a hash of (seed, step,
 // number of the element): no state, no order, the same on every run.  A scale that is a power of two decodes exactly, and what
-// was decoded encodes to itself, so a checkpoint in float32 resumes where it was.  A block with a NaN or an infinity has the
-// exponent byte 255 and decodes to NaN as a whole.
+// was decoded encodes to itself, so a checkpoint in float32 resumes where it was.  A block with a NaN, an infinity or a magnitude
+// above 1.875 * 2^127 (whose exponent would be 255) has the exponent byte 255 and decodes to NaN as a whole.
 //
 // What bounds it: memory.  Every value is read and written once: 28 bytes with float32 moments, 16 with 8-bit ones.  256 M float32
 // values take 1.39 ms, 5.15 TB/s; four arrays read and three written at once is what costs against the 5.9 TB/s of one array scaled

@@ -527,3 +527,20 @@ def test_rates_and_eps_at_the_ends_bit_for_bit(T, lr, eps):
         opt.step()
         ref.step([g])
         same(p, ref.p[0], 'p, step %d' % step)
+
+
+def test_largest_magnitude_of_a_block(T):
+    """Up to 1.875 * 2^127 a value has its place; a block with a larger one becomes NaN like one with an infinity."""
+    big = np.float32(1.875 * 2.0 ** 127)
+    m = np.zeros(768, np.float32)
+    m[3], m[300], m[600] = big, np.nextafter(big, np.float32(np.inf)), -big
+    v = np.zeros(768, np.float32)
+    v[5], v[301], v[700] = np.nextafter(big, np.float32(np.inf)), 1.0, big
+    p = nn.Parameter(torch.zeros(768, device='cuda'))
+    opt = T.AdamW([p], state_bits=8, **HP)
+    opt.load_state_dict({'state': {0: {'step': 1, 'exp_avg': f32(m), 'exp_avg_sq': f32(v)}}, 'param_groups': opt.state_dict()['param_groups']})
+    m[256:512] = np.nan
+    v[:256] = np.nan
+    a, b = opt.moments()
+    same(a, m, 'm')
+    same(b, v, 'v')
