@@ -9,8 +9,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 SOURCES = ['layout.hip', 'fbm.hip', 'fbm_fast.hip', 'fbm_fast_mixed.hip', 'fbm_mfma.hip', 'gates.hip', 'weightgen.hip', 'weightgen_bwd.hip', 'conv.hip', 'conv_plain.hip', 'net.hip', 'head.hip', 'train.hip', 'adamw.hip']
-# no packed float32 instructions: some of their forms have given wrong results on gfx950 now and then, and they gain nothing here
-# (batch of 16 512x512 images: 692.9 and 694.0 ms with them, 692.7 and 693.4 ms without)
+# no packed float32 instructions: some of their forms have given wrong results on gfx950 now and then
+# (measured on a batch of 16 512x512 images, 692.9 and 694.0 ms with them, 692.7 and 693.4 without, and on the training step; the tiled,
+# plain and SRVGG workloads were not compared)
 FLAGS = ['-O3', '--offload-arch=gfx950', '-std=c++17', '-fno-signed-zeros', '-fPIC', '-Wall', '-Wno-unused-result', '-Xclang', '-target-feature', '-Xclang',
          '-packed-fp32-ops']
 # adamw.hip: every operation rounded once (its results are those of the formulas, bit for bit)

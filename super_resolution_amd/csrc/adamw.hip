@@ -22,7 +22,7 @@
 // What bounds it: memory.  Every value is read and written once: 28 bytes with float32 moments, 16 with 8-bit ones.  256 M float32
 // values take 1.39 ms, 5.15 TB/s; four arrays read and three written at once is what costs against the 5.9 TB/s of one array scaled
 // in place (5.65 for three read and one written): with the arithmetic taken out the time is the same.  8-bit moments: 128 M float32
-// values 0.39 ms, 5.2 TB/s; with bfloat16 weights (10 bytes, 76 vector instructions a value) 96 M take 0.19 to 0.25 ms, and their
+// values 0.40 ms, 5.15 TB/s; with bfloat16 weights (10 bytes, 76 vector instructions a value) 96 M take 0.20 to 0.24 ms, and their
 // instructions alone 0.19 to issue.
 // Work is split into pieces of 1024 consecutive values of one tensor, one per WAVE: most of RRDBNet-FDConv's 8380 tensors are
 // smaller than a piece, and a workgroup each would leave three of its four waves idle.  A wave issues the loads of its four groups
@@ -75,6 +75,7 @@ struct Scalars {
 };
 
 __host__ __device__ inline void make_key(uint64_t seed, int64_t step, Scalars& s) {  // splitmix64
+    // (G. Steele, D. Lea, C. Flood, "Fast splittable pseudorandom number generators", 2014)
     uint64_t z = seed + (uint64_t)step * 0x9E3779B97F4A7C15ull;
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
     z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
@@ -98,8 +99,8 @@ __host__ __device__ inline Scalars make_scalars(const sr_adamw_hyper& h, double 
     return s;
 }
 
-// 32 random bits for element (hi, lo) of a step; hi_c = hi * GOLDEN.  The two odd constants and the shifts are a published
-// full-avalanche mixer of 32-bit words; k1 enters between them so that steps whose k0 differ in few bits do not share values.
+// 32 random bits for element (hi, lo) of a step; hi_c = hi * GOLDEN.  The two odd constants and the shifts are those of the mixer of
+// 32-bit words with the least bias that Christopher Wellons found by search and published in 2018; k1 enters between them so that steps whose k0 differ in few bits do not share values.
 __device__ __forceinline__ uint32_t mix(uint32_t lo, uint32_t hi_c, uint32_t k0, uint32_t k1) {
     uint32_t x = (lo ^ k0) + hi_c;
     x = (x ^ (x >> 16)) * 0x7FEB352Du + k1;
