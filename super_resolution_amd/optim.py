@@ -397,7 +397,8 @@ class AdamW(torch.optim.Optimizer):
         loss.backward()
         opt.step(clip_grad_norm=1.0)          # or train.train_step(net, opt, ...)
 
-    Parameters: float32 or bfloat16, dense, on one GPU; they stay where they are.  bfloat16 parameters are rounded
+    Parameters: float32 or bfloat16, dense, on one GPU; they stay where they are.  Re-pointed ones (`.data =`) of the same dtype, device and
+    shape are followed, element by element where the order in memory changes.  bfloat16 parameters are rounded
     stochastically (an update of 1e-4 of a weight is below half a bfloat16 step and would be lost).  8-bit moments: 256 values share an
     exponent byte, m and v have three mantissa bits each and are rounded stochastically (rounded to nearest, v would not move under
     beta2 = 0.999); 2.01 bytes of state a parameter instead of 8.  The random bits are a hash of (seed, step, element): two runs
@@ -451,7 +452,7 @@ class AdamW(torch.optim.Optimizer):
         self._index, self._block = before(size), before(in_blocks)
         self._at = np.where(bits == 8, before(in_8), before(in_32))
         n, blocks = {32: int(in_32.sum()), 8: int(in_8.sum())}, int(in_blocks.sum())
-        self.numel = total = int(size.sum())
+        self.numel, self._sizes = int(size.sum()), size.tolist()
         with torch.cuda.device(dev), torch.no_grad():
             if broadcast and _world(group) > 1:
                 _broadcast_parameters(self.params, group)
@@ -460,7 +461,7 @@ class AdamW(torch.optim.Optimizer):
             self._me, self._ve = (torch.ones(blocks, dtype=torch.uint8, device=dev) for _ in range(2))
             self.ema = None
             if ema_decay is not None:
-                self.ema = torch.empty(total, dtype=torch.float32, device=dev)
+                self.ema = torch.empty(self.numel, dtype=torch.float32, device=dev)
                 self._reset_ema()
             self._lists, first = [], 0
             for k, g in enumerate(self.param_groups):
@@ -518,7 +519,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _shaped(self, flat):
         """The parameters' parts of a flat array, with the elements at the parameters' indices."""
-        parts = flat.split([p.numel() for p in self.params])
+        parts = flat.split(self._sizes)
         return [x.as_strided(shape, self._stride[i]) if i in self._stride else x.view(shape) for i, (x, shape) in enumerate(zip(parts, self._shape))]
 
     @property
@@ -817,10 +818,9 @@ class AdamW(torch.optim.Optimizer):
             mine.update(hp)
 
         def part(name, i):
-            p, stride = self.params[i], self._stride.get(i)
-            x = state.get(i, {}).get(name, p if name == 'ema' else None)
+            stride, x = self._stride.get(i), state.get(i, {}).get(name, self.params[i] if name == 'ema' else None)
             if x is None:
-                return torch.zeros(p.numel(), dtype=torch.float32, device=self.device)
+                return torch.zeros(self._sizes[i], dtype=torch.float32, device=self.device)
             if x.dtype != torch.float32 or x.device != self.device:
                 x = x.to(self.device, torch.float32)
             if stride is None:

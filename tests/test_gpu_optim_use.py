@@ -544,3 +544,20 @@ def test_largest_magnitude_of_a_block(T):
     a, b = opt.moments()
     same(a, m, 'm')
     same(b, v, 'v')
+
+
+def test_checkpoints_beside_a_resized_parameter(T):
+    """Refused by the step, a parameter of another size does not shift what is saved and loaded for the others."""
+    p, q = nn.Parameter(torch.ones(5, 4, device='cuda')), nn.Parameter(torch.ones(300, device='cuda'))
+    opt = T.AdamW([p, q], ema_decay=0.9)
+    p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+    opt.step()
+    want = copy.deepcopy(opt.state_dict())
+    p.data, p.grad = torch.ones(9, 7, device='cuda'), None
+    with pytest.raises(RuntimeError, match='rebuild'):
+        opt.step()
+    for _ in range(2):
+        got = opt.state_dict()
+        for i in range(2):
+            assert all(torch.equal(got['state'][i][k], want['state'][i][k]) for k in ('exp_avg', 'exp_avg_sq', 'ema'))
+        opt.load_state_dict(want)
